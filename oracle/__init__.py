@@ -54,8 +54,8 @@ _u16p = ctypes.POINTER(ctypes.c_uint16)
 
 def reference_dir() -> str | None:
     """Where the reference's sources are: the STLQ_REF_DIR environment variable, else the
-    ``reference_path`` recorded in the repository's BASELINE.json.  None when neither names an
-    existing directory (a GPU box, which only uses the prebuilt libraries)."""
+    ``reference_path`` recorded in the repository's BASELINE.json.  None when neither names a
+    directory that holds them (a GPU box, which only uses the prebuilt libraries)."""
     cand = os.environ.get("STLQ_REF_DIR")
     if not cand:
         try:
@@ -65,7 +65,7 @@ def reference_dir() -> str | None:
                 cand = json.load(f).get("reference_path")
         except (OSError, ValueError):
             cand = None
-    return cand if cand and os.path.isdir(cand) else None
+    return cand if cand and os.path.isdir(os.path.join(cand, "src")) else None
 
 
 def build(reference: bool = True) -> None:
