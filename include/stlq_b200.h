@@ -47,15 +47,19 @@ enum {
     STLQ_B200_GEMM_FAST = 2
 };
 
-/* Input element types for X. */
-enum { STLQ_B200_F32 = 0, STLQ_B200_U8 = 1 };
+/* Input element types for X.  The routed 8-bit operators at the end of this file also take the others;
+ * the encode entry points take the first two. */
+enum { STLQ_B200_F32 = 0, STLQ_B200_U8 = 1, STLQ_B200_BF16 = 2, STLQ_B200_F16 = 3, STLQ_B200_I32 = 4, STLQ_B200_I64 = 5 };
 
 /* Limits of this build. */
 #define STLQ_B200_MAX_M 16      /* codebooks (layers) */
 #define STLQ_B200_MAX_K 256     /* codewords per codebook with uint8 codes */
 #define STLQ_B200_MAX_K_WIDE 1024 /* codewords per codebook with uint16 codes (the _u16 entry points) */
 #define STLQ_B200_MAX_BEAM 32   /* beam width */
-#define STLQ_B200_MAX_ROOT 65536 /* root codewords of a large-root encoder */
+#define STLQ_B200_MAX_ROOT 65536 /* root codewords of a large-root encoder; experts of a sort or an exchange */
+#define STLQ_B200_MAX_TOPK 64     /* choices (experts) of one row */
+#define STLQ_B200_MAX_EXPERTS 1024 /* matrices of one grouped product */
+#define STLQ_B200_MAX_I8_K 131071 /* terms of an 8-bit product's sum (a 32-bit integer holds it exactly) */
 
 /* Message for the last failed call on this host thread ("" if none). */
 const char* stlq_b200_last_error(void);
@@ -346,6 +350,77 @@ int stlq_b200_u8_to_f32(stlq_b200_kernels* k, const uint8_t* in, int ld_in, int 
  * idx or val may be NULL. */
 int stlq_b200_argmax_cols(stlq_b200_kernels* k, const float* scores, int ld, int rows, int64_t cols, int* idx,
                           float* val, void* stream);
+
+/* ---- Routed 8-bit operators ----
+ * What follows an assignment of vectors (rows, tokens) to root codewords (experts): bring the rows of
+ * an expert together, take them through that expert's matrix in 8-bit integers, and bring the results
+ * back with weights; and the gradient of the exchange.  The reference has no counterpart.
+ *
+ * Matrices here are row-major with a leading dimension in elements: row r starts at p + r * ld.  All
+ * pointers are on the handle's device and aligned to their elements; calls are asynchronous on
+ * `stream`, allocate nothing, keep nothing between calls and may be captured in a CUDA graph.  Outputs
+ * must not overlap inputs.  "FLOAT" stands for STLQ_B200_F32, _BF16 or _F16.  A value is rounded to
+ * a 16-bit type once, when it is written. */
+
+/* q = the rows of x in 8 bits, scale = their scales: scale[r] = max_c |x[r, c]| / 127 and
+ * q[r, c] = 127 x[r, c] / max_c |x[r, c]| rounded to the nearest integer (ties to even), both in 32 bits.  A row of
+ * zeros has scale 0; a row with an infinity or a NaN has scale NaN and q = 0, so that its products are NaN.  x: FLOAT.
+ * It also lays out the weights of the products below, one row and one scale per channel. */
+int stlq_b200_quantize_rows(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int64_t rows, int cols,
+                            int8_t* q, int64_t ldq, float* scale, void* stream);
+
+/* out[r, c] = (sum_i q[r, i] w[c, i]) q_scale[r] w_scale[c] + bias[c], the sum exact, the rest in 32 bits; bias may be
+ * NULL.  q: rows x kdim, w: n x kdim, out: rows x n (FLOAT).  q and w 16-byte aligned, ldq and ldw multiples of 16;
+ * bytes of a row past kdim are not used.  kdim 0 gives the bias, or zeros. */
+int stlq_b200_matmul_i8(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_scale, const int8_t* w,
+                        int64_t ldw, const float* w_scale, const float* bias, int64_t rows, int n, int kdim, void* out,
+                        int out_dtype, int64_t ldo, void* stream);
+
+/* The same product where row r in [offsets[e], offsets[e + 1]) takes expert e's matrix: w (experts * n) x kdim,
+ * expert e's channels at rows e n .. e n + n - 1, w_scale and bias likewise.  offsets: experts + 1 on the device, as
+ * stlq_b200_sort_by_expert writes them.  Rows from offsets[experts] on are zeros. */
+int stlq_b200_matmul_i8_grouped(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_scale, const int8_t* w,
+                                int64_t ldw, const float* w_scale, const float* bias, const int32_t* offsets, int experts,
+                                int64_t rows, int n, int kdim, void* out, int out_dtype, int64_t ldo, void* stream);
+
+/* The pairs p = t * topk + j of ids (tokens x topk, contiguous, STLQ_B200_I32 or _I64) sorted by expert, in the order of
+ * p within an expert: order[r] = the pair at sorted row r, position[p] = the sorted row of pair p, offsets[e] = the first
+ * row of expert e (experts + 1 values; offsets[experts] = rows kept).  An id outside [0, experts) is a dropped choice:
+ * its pair comes after all kept ones.  tokens * topk below 2^31.  workspace: 16-byte aligned, of the bytes that
+ * stlq_b200_sort_by_expert_workspace gives; free again once the call's work is done. */
+int stlq_b200_sort_by_expert_workspace(int64_t tokens, int topk, int experts, size_t* bytes);
+int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtype, int64_t tokens, int topk, int experts,
+                             int32_t* order, int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* Rows to their experts: out[position[t, j]] = x[t], zeros where the choice was dropped; out has tokens * topk rows.
+ * Elements of 1, 2 or 4 bytes, copied as they are. */
+int stlq_b200_dispatch(stlq_b200_kernels* k, const void* x, int elem_bytes, int64_t ldx, int64_t tokens, int cols, int topk,
+                       const int32_t* position, const int32_t* offsets, int experts, void* out, int64_t ldo, void* stream);
+
+/* stlq_b200_quantize_rows and stlq_b200_dispatch in one: q and scale have tokens * topk rows. */
+int stlq_b200_dispatch_i8(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int64_t tokens, int cols, int topk,
+                          const int32_t* position, const int32_t* offsets, int experts, int8_t* q, int64_t ldq,
+                          float* scale, void* stream);
+
+/* Back from the experts: out[t] = sum over the kept choices of weights[t, j] y[position[t, j]], in 32 bits, j ascending;
+ * zeros for a token with none.  Rows of dropped choices are not read.  y and out: FLOAT (one type); weights:
+ * tokens x topk, contiguous, FLOAT, or NULL for ones, which is the gradient of stlq_b200_dispatch. */
+int stlq_b200_combine(stlq_b200_kernels* k, const void* y, int dtype, int64_t ldy, int64_t tokens, int cols, int topk,
+                      const void* weights, int weights_dtype, const int32_t* position, const int32_t* offsets, int experts,
+                      void* out, int64_t ldo, void* stream);
+
+/* The gradient of stlq_b200_combine: dy[position[t, j]] = weights[t, j] dout[t] and
+ * dweights[t, j] = <dout[t], y[position[t, j]]>; both zero where the choice was dropped.  dout, y and dy: one FLOAT type;
+ * dweights has the weights' type. */
+int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype, int64_t ldd, const void* y, int64_t ldy,
+                               int64_t tokens, int cols, int topk, const void* weights, int weights_dtype,
+                               const int32_t* position, const int32_t* offsets, int experts, void* dy, int64_t lddy,
+                               void* dweights, void* stream);
+
+/* Waits for the work enqueued on `stream`; STLQ_B200_EDEVICE if a kernel of this handle reported an error since the
+ * last call (a product whose bounded waits ran out). */
+int stlq_b200_kernels_sync(stlq_b200_kernels* k, void* stream);
 
 /* Block until all work this encoder enqueued on `stream` has finished; returns
  * STLQ_B200_EDEVICE if a kernel flagged an internal error since the last check. */

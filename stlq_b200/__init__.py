@@ -17,3 +17,4 @@ from .encoder import (  # noqa: F401
     library_path,
     load_library,
 )
+from .operators import Kernels, Routing  # noqa: F401

@@ -5,15 +5,16 @@
 // on top of these.
 #include <algorithm>
 #include <cstdint>
+#include <new>
 #include <string>
 
 #include <cuda_runtime.h>
 
 #include "../../include/stlq_b200.h"
 #include "launch.h"
+#include "provider.h"
 
 namespace stlq_b200 {
-int SetError(int code, const char* msg);
 cudaError_t LaunchSgemmExact(const float* A, int64_t lda, int rows, int k, const float* B, int64_t ldb, int64_t n,
                              float alpha, float beta, float* out, int ldo, cudaStream_t stream);
 }  // namespace stlq_b200
@@ -90,56 +91,12 @@ __global__ void ArgmaxColsKernel(const float* __restrict__ scores, int64_t ld, i
     }
 }
 
-int Ck(cudaError_t e, const char* what) {
-    if (e == cudaSuccess) return 0;
-    cudaGetLastError();
-    return stlq_b200::SetError(e == cudaErrorMemoryAllocation ? STLQ_B200_ENOMEM : STLQ_B200_ECUDA,
-                               (std::string(what) + ": " + cudaGetErrorString(e)).c_str());
-}
-
-struct Scratch {
-    void* p = nullptr;
-    size_t bytes = 0;
-    int Ensure(size_t need) {
-        if (need <= bytes) return 0;
-        if (p) cudaFree(p);
-        p = nullptr;
-        bytes = 0;
-        if (int rc = Ck(cudaMalloc(&p, need), "cudaMalloc (kernel-provider scratch)")) return rc;
-        bytes = need;
-        return 0;
-    }
-    void Release() {
-        if (p) cudaFree(p);
-        p = nullptr;
-        bytes = 0;
-    }
-};
-
-class DeviceScope {
-public:
-    explicit DeviceScope(int device) {
-        if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
-        ok_ = cudaSetDevice(device) == cudaSuccess;
-    }
-    ~DeviceScope() {
-        if (prev_ >= 0) cudaSetDevice(prev_);
-    }
-    bool ok() const { return ok_; }
-
-private:
-    int prev_ = -1;
-    bool ok_ = false;
-};
-
 int GridFor(int64_t total) { return static_cast<int>(std::min<int64_t>((total + 255) / 256, 148 * 32)); }
 
 }  // namespace
 
-struct stlq_b200_kernels {
-    int device = 0;
-    Scratch At, Bt;  // op(A) rows / op(B) columns made contiguous when the operand layout needs it
-};
+using stlq_b200::Ck;
+using stlq_b200::DeviceScope;
 
 extern "C" {
 
@@ -149,10 +106,37 @@ int stlq_b200_kernels_create(int device, stlq_b200_kernels** out) {
     int ndev = 0;
     if (int rc = Ck(cudaGetDeviceCount(&ndev), "cudaGetDeviceCount")) return rc;
     if (device < 0 || device >= ndev) return stlq_b200::SetError(STLQ_B200_EINVAL, "device ordinal out of range");
-    auto* k = new stlq_b200_kernels();
+    auto* k = new (std::nothrow) stlq_b200_kernels();
+    if (!k) return stlq_b200::SetError(STLQ_B200_ENOMEM, "out of host memory");
     k->device = device;
+    DeviceScope scope(device);
+    int rc = scope.ok() ? 0 : stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+    if (!rc) rc = Ck(cudaDeviceGetAttribute(&k->num_sms, cudaDevAttrMultiProcessorCount, device), "multiprocessor count");
+    if (!rc) rc = k->err.Ensure(sizeof(unsigned int));
+    if (!rc) rc = Ck(cudaMemset(k->err.p, 0, sizeof(unsigned int)), "cudaMemset");
+    if (!rc) rc = Ck(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize");  // before work on any other stream
+    if (rc) {
+        k->err.Release();
+        delete k;
+        return rc;
+    }
     *out = k;
     return 0;
+}
+
+int stlq_b200_kernels_sync(stlq_b200_kernels* k, void* stream) {
+    if (!k) return stlq_b200::SetError(STLQ_B200_EINVAL, "kernel-provider handle is null");
+    DeviceScope scope(k->device);
+    if (!scope.ok()) return stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    unsigned int flags = 0;
+    if (int rc = Ck(cudaMemcpyAsync(&flags, k->err.p, sizeof(flags), cudaMemcpyDeviceToHost, s), "error flag")) return rc;
+    if (int rc = Ck(cudaStreamSynchronize(s), "cudaStreamSynchronize")) return rc;
+    if (!flags) return 0;
+    if (int rc = Ck(cudaMemsetAsync(k->err.p, 0, sizeof(flags), s), "error flag")) return rc;
+    return stlq_b200::SetError(STLQ_B200_EDEVICE, flags & stlq_b200::kErrWaitTimeout
+                                                      ? "a kernel's bounded wait expired: its results are not valid"
+                                                      : "a kernel reported an internal error");
 }
 
 int stlq_b200_kernels_destroy(stlq_b200_kernels* k) {
@@ -160,6 +144,7 @@ int stlq_b200_kernels_destroy(stlq_b200_kernels* k) {
     DeviceScope scope(k->device);
     k->At.Release();
     k->Bt.Release();
+    k->err.Release();
     delete k;
     return 0;
 }

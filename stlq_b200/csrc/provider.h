@@ -1,0 +1,67 @@
+// The kernel-provider handle and the host helpers its entry points share (provider.cu, routed.cu,
+// matmul_i8.cu).
+#pragma once
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+#include <string>
+
+#include <cuda_runtime.h>
+
+#include "../../include/stlq_b200.h"
+
+namespace stlq_b200 {
+int SetError(int code, const char* msg);
+
+inline int Ck(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return 0;
+    cudaGetLastError();
+    return SetError(e == cudaErrorMemoryAllocation ? STLQ_B200_ENOMEM : STLQ_B200_ECUDA,
+                    (std::string(what) + ": " + cudaGetErrorString(e)).c_str());
+}
+
+struct Scratch {
+    void* p = nullptr;
+    size_t bytes = 0;
+    int Ensure(size_t need) {
+        if (need <= bytes) return 0;
+        if (p) cudaFree(p);
+        p = nullptr;
+        bytes = 0;
+        if (int rc = Ck(cudaMalloc(&p, need), "cudaMalloc (kernel-provider scratch)")) return rc;
+        bytes = need;
+        return 0;
+    }
+    void Release() {
+        if (p) cudaFree(p);
+        p = nullptr;
+        bytes = 0;
+    }
+};
+
+class DeviceScope {
+public:
+    explicit DeviceScope(int device) {
+        if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+        ok_ = prev_ == device || cudaSetDevice(device) == cudaSuccess;
+        restore_ = prev_ >= 0 && prev_ != device;
+    }
+    ~DeviceScope() {
+        if (restore_) cudaSetDevice(prev_);
+    }
+    bool ok() const { return ok_; }
+
+private:
+    int prev_ = -1;
+    bool ok_ = false, restore_ = false;
+};
+
+}  // namespace stlq_b200
+
+struct stlq_b200_kernels {
+    int device = 0;
+    int num_sms = 148;
+    stlq_b200::Scratch At, Bt;  // op(A) rows / op(B) columns made contiguous when the operand layout needs it
+    stlq_b200::Scratch err;     // one word: kernels OR DeviceError bits into it (stlq_b200_kernels_sync reads it)
+};

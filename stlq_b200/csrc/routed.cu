@@ -1,0 +1,745 @@
+// Rows quantised to 8 bits, rows sorted by the expert (or root codeword) they were assigned to and
+// back, with weights applied, and the gradient of that exchange.
+//
+// T tokens (rows) with k choices of E experts make P = T k pairs; pair p = t k + j.  A choice outside
+// [0, E) is dropped.  order is the stable sort of the pairs by expert, dropped pairs last; position
+// its inverse; offsets[e] the first sorted row of expert e, offsets[E] the rows kept.  Every kernel
+// compares a position with offsets[E] and with P before it uses it, so arrays that no sort made
+// cannot lead outside a buffer.  Nothing here accumulates through atomics in an order that matters:
+// results do not change from call to call.
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "provider.h"
+
+namespace {
+
+using stlq_b200::Ck;
+using stlq_b200::DeviceScope;
+using stlq_b200::SetError;
+
+constexpr int kBlock = 256;
+
+template <typename T>
+__device__ __forceinline__ float ToFloat(T v) {
+    if constexpr (std::is_same_v<T, float>) return v;
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
+    else return __half2float(v);
+}
+template <typename T>
+__device__ __forceinline__ T FromFloat(float v) {
+    if constexpr (std::is_same_v<T, float>) return v;
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+    else return __float2half_rn(v);
+}
+
+// N consecutive elements moved as one access (N * sizeof(T) bytes, aligned to as many).
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+__device__ __forceinline__ float LoadAs(const void* p, int64_t i, int dtype) {
+    if (dtype == STLQ_B200_F32) return static_cast<const float*>(p)[i];
+    if (dtype == STLQ_B200_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void StoreAs(void* p, int64_t i, int dtype, float v) {
+    if (dtype == STLQ_B200_F32) static_cast<float*>(p)[i] = v;
+    else if (dtype == STLQ_B200_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// offsets[E] as the kernels use it: rows kept, within [0, P].
+__device__ __forceinline__ int Kept(const int* offsets, int experts, int pairs) {
+    return min(max(__ldg(offsets + experts), 0), pairs);
+}
+
+// ---- quantisation of rows ----------------------------------------------------------------------
+
+// 127 x / amax in 32 bits (two roundings), to the nearest integer, ties to even.  `down` keeps 127 x
+// finite for the largest rows: both are multiplied by 2^-8, which changes no bit of the quotient.
+__device__ __forceinline__ int Quantise(float x, float amax, float down) {
+    return __float2int_rn(__fdiv_rn(__fmul_rn(__fmul_rn(x, down), 127.0f), __fmul_rn(amax, down)));
+}
+
+// One group of L threads quantises one row and writes it once (position null) or to the rows of its
+// choices.  The row is read once: a thread keeps its first kHold vectors in registers between the
+// maximum and the rounding, and re-reads the rest.
+constexpr int kHold = 4;
+
+template <typename T, int N, int L>
+__global__ void __launch_bounds__(kBlock)
+    QuantizeRowsKernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int topk,
+                       const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
+                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
+    constexpr int kGroups = kBlock / L;
+    __shared__ unsigned int part[kBlock / 32];
+    const int group = threadIdx.x / L, at = threadIdx.x % L;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+    const bool real = row < rows;
+    const int full = cols / N;
+    const T* xr = x + (real ? row : 0) * ldx;
+    Pack<T, N> hold[kHold];
+    // The largest |x| by its bits: unsigned order puts every NaN above infinity above the numbers.
+    unsigned int top = 0;
+    if (real) {
+#pragma unroll
+        for (int h = 0; h < kHold; ++h) {
+            const int c = at + h * L;
+            if (c >= full) break;
+            hold[h] = *reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N);
+#pragma unroll
+            for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(ToFloat(hold[h].v[i])) & 0x7fffffffu);
+        }
+        for (int c = at + kHold * L; c < full; c += L) {
+            const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N);
+#pragma unroll
+            for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(ToFloat(v.v[i])) & 0x7fffffffu);
+        }
+        for (int c = full * N + at; c < cols; c += L) top = max(top, __float_as_uint(ToFloat(xr[c])) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (L > 32) {
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < L / 32; ++w) top = max(top, part[group * (L / 32) + w]);
+    }
+    if (!real) return;
+    const float amax = __uint_as_float(top);
+    const bool finite = top < 0x7f800000u;
+    const bool some = finite && top != 0;
+    const float down = amax > 1e36f ? 0.00390625f : 1.0f;
+    const float s = finite ? __fdiv_rn(amax, 127.0f) : __int_as_float(0x7fc00000);
+    const int kept = position ? Kept(offsets, experts, pairs) : 0;
+    const int copies = position ? topk : 1;
+    auto target = [&](int j) -> int64_t {
+        if (!position) return row;
+        const int p = __ldg(position + row * topk + j);
+        return static_cast<unsigned>(p) < static_cast<unsigned>(pairs) ? p : -1;
+    };
+    // Dropped choices get a row of zeros with scale 0.
+    auto store = [&](int c, const Pack<T, N>& v) {
+        Pack<int8_t, N> r, zero;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            r.v[i] = some ? static_cast<int8_t>(Quantise(ToFloat(v.v[i]), amax, down)) : static_cast<int8_t>(0);
+            zero.v[i] = 0;
+        }
+        for (int j = 0; j < copies; ++j) {
+            const int64_t to = target(j);
+            if (to >= 0)
+                *reinterpret_cast<Pack<int8_t, N>*>(q + to * ldq + static_cast<int64_t>(c) * N) =
+                    (!position || to < kept) ? r : zero;
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < kHold; ++h) {
+        const int c = at + h * L;
+        if (c >= full) break;
+        store(c, hold[h]);
+    }
+    for (int c = at + kHold * L; c < full; c += L)
+        store(c, *reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N));
+    for (int c = full * N + at; c < cols; c += L) {
+        const int8_t r = some ? static_cast<int8_t>(Quantise(ToFloat(xr[c]), amax, down)) : static_cast<int8_t>(0);
+        for (int j = 0; j < copies; ++j) {
+            const int64_t to = target(j);
+            if (to >= 0) q[to * ldq + c] = (!position || to < kept) ? r : static_cast<int8_t>(0);
+        }
+    }
+    for (int j = at; j < copies; j += L) {
+        const int64_t to = target(j);
+        if (to >= 0) scale[to] = (!position || to < kept) ? s : 0.0f;
+    }
+}
+
+// ---- sort by expert ----------------------------------------------------------------------------
+
+// A counting sort over `bins` digits, stable: a tile of kTile keys per block, each of its warps
+// ranking a contiguous piece 32 keys at a time (__match_any_sync gives the lanes that share a
+// digit).  Up to kOneBins - 1 experts it is one pass; above that two passes of half the key's bits
+// each, from the low digit to the high one.
+constexpr int kSortBlock = 512;
+constexpr int kSortWarps = kSortBlock / 32;
+constexpr int kPerWarp = 256;
+constexpr int kTile = kSortWarps * kPerWarp;
+constexpr int kOneBins = 1025;
+
+struct SortPass {
+    const void* ids;   // first pass: the caller's ids
+    int wide;          // ids are int64
+    const int* keys;   // second pass: the keys and pairs that the first pass left
+    const int* pairs;
+    int n, experts, shift, mask, bins, tiles;
+};
+
+__device__ __forceinline__ int KeyOf(const SortPass& a, int i) {
+    if (a.keys) return a.keys[i];
+    const int64_t id = a.wide ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int*>(a.ids)[i];
+    return id >= 0 && id < a.experts ? static_cast<int>(id) : a.experts;
+}
+
+// Digits of this warp's keys counted into count[bins]; kRank: each key's rank among the warp's keys
+// of its digit goes to rank[].
+template <bool kRank>
+__device__ __forceinline__ void CountWarp(const SortPass& a, int first, unsigned short* count, unsigned short* rank) {
+    const int lane = threadIdx.x & 31;
+    for (int r = 0; r < kPerWarp / 32; ++r) {
+        const int i = first + r * 32 + lane;
+        const int d = i < a.n ? (KeyOf(a, i) >> a.shift) & a.mask : a.bins;  // no key: a digit of its own
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const int before = d < a.bins ? count[d] : 0;
+        const int mine = __popc(same & ((1u << lane) - 1));
+        if (kRank) rank[r] = static_cast<unsigned short>(before + mine);
+        __syncwarp();
+        if (mine == 0 && d < a.bins) count[d] = static_cast<unsigned short>(before + __popc(same));
+        __syncwarp();
+    }
+}
+
+__global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* __restrict__ hist, int* __restrict__ totals) {
+    extern __shared__ unsigned short counts[];  // [kSortWarps][bins]
+    for (int i = threadIdx.x; i < kSortWarps * a.bins; i += kSortBlock) counts[i] = 0;
+    __syncthreads();
+    const int warp = threadIdx.x >> 5;
+    CountWarp<false>(a, blockIdx.x * kTile + warp * kPerWarp, counts + warp * a.bins, nullptr);
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.bins; b += kSortBlock) {
+        int sum = 0;
+        for (int w = 0; w < kSortWarps; ++w) sum += counts[w * a.bins + b];
+        hist[static_cast<int64_t>(b) * a.tiles + blockIdx.x] = sum;
+    }
+    if (totals)  // two-pass sorts: keys per expert (whole numbers, so the order of the additions is free)
+        for (int i = blockIdx.x * kTile + threadIdx.x; i < min(a.n, (static_cast<int>(blockIdx.x) + 1) * kTile); i += kSortBlock)
+            atomicAdd(totals + KeyOf(a, i), 1);
+}
+
+// Exclusive scan of n counters by one block.
+__device__ void ScanBlock(int* v, int64_t n) {
+    __shared__ int part[32];
+    __shared__ int carry;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (threadIdx.x == 0) carry = 0;
+    __syncthreads();
+    for (int64_t base = 0; base < n; base += blockDim.x) {
+        const int64_t i = base + threadIdx.x;
+        const int x = i < n ? v[i] : 0;
+        int s = x;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += y;
+        }
+        if (lane == 31) part[warp] = s;
+        __syncthreads();
+        if (warp == 0) {
+            int t = lane < warps ? part[lane] : 0;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, t, o);
+                if (lane >= o) t += y;
+            }
+            part[lane] = t;
+        }
+        __syncthreads();
+        const int before = carry + (warp ? part[warp - 1] : 0);
+        if (i < n) v[i] = before + s - x;
+        const int all = part[warps - 1];
+        __syncthreads();
+        if (threadIdx.x == 0) carry += all;
+        __syncthreads();
+    }
+}
+
+// Block 0 scans the counters of a pass; block 1, when there is one, the keys per expert.
+__global__ void __launch_bounds__(1024) SortScanKernel(int* __restrict__ hist, int64_t n, int* __restrict__ totals, int64_t m) {
+    if (blockIdx.x == 0) ScanBlock(hist, n);
+    else ScanBlock(totals, m);
+}
+
+// offsets (one-pass sorts) are the counters of each digit's first tile.
+__global__ void __launch_bounds__(kSortBlock)
+    SortScatterKernel(SortPass a, const int* __restrict__ hist, int* __restrict__ keys_out, int* __restrict__ pairs_out,
+                      int* __restrict__ position, int* __restrict__ offsets) {
+    extern __shared__ unsigned short counts[];  // [kSortWarps][bins], then [bins] ints
+    int* base = reinterpret_cast<int*>(counts + ((kSortWarps * a.bins + 1) & ~1));
+    for (int i = threadIdx.x; i < kSortWarps * a.bins; i += kSortBlock) counts[i] = 0;
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int first = blockIdx.x * kTile + warp * kPerWarp;
+    unsigned short rank[kPerWarp / 32];
+    CountWarp<true>(a, first, counts + warp * a.bins, rank);
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.bins; b += kSortBlock) {
+        int sum = 0;
+        for (int w = 0; w < kSortWarps; ++w) {
+            const int c = counts[w * a.bins + b];
+            counts[w * a.bins + b] = static_cast<unsigned short>(sum);
+            sum += c;
+        }
+        base[b] = hist[static_cast<int64_t>(b) * a.tiles + blockIdx.x];
+        if (offsets && blockIdx.x == 0) offsets[b] = base[b];
+    }
+    __syncthreads();
+    for (int r = 0; r < kPerWarp / 32; ++r) {
+        const int i = first + r * 32 + lane;
+        if (i >= a.n) break;
+        const int key = KeyOf(a, i), d = (key >> a.shift) & a.mask;
+        const int to = base[d] + counts[warp * a.bins + d] + rank[r];
+        const int pair = a.pairs ? a.pairs[i] : i;
+        pairs_out[to] = pair;
+        if (keys_out) keys_out[to] = key;
+        if (position) position[pair] = to;
+    }
+}
+
+__global__ void NoPairsKernel(int* offsets, int n) {
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) offsets[i] = 0;
+}
+
+struct SortPlan {
+    int bins[2], shift[2], passes, tiles;
+    size_t hist, keys, pairs, totals, bytes;  // places in the workspace
+};
+
+SortPlan PlanSort(int64_t n, int experts) {
+    SortPlan p{};
+    p.tiles = static_cast<int>((n + kTile - 1) / kTile);
+    if (experts + 1 <= kOneBins) {
+        p.passes = 1;
+        p.bins[0] = experts + 1;
+    } else {
+        int bits = 1;
+        while ((experts >> bits) != 0) ++bits;
+        p.passes = 2;
+        p.shift[1] = (bits + 1) / 2;
+        p.bins[0] = 1 << p.shift[1];
+        p.bins[1] = (experts >> p.shift[1]) + 1;
+    }
+    const auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
+    const size_t most = std::max(p.bins[0], p.bins[1]);
+    p.keys = up(most * p.tiles * sizeof(int));
+    p.pairs = p.keys;
+    p.totals = p.keys;
+    p.bytes = p.keys;
+    if (p.passes == 2) {
+        p.pairs = p.keys + up(static_cast<size_t>(n) * sizeof(int));
+        p.totals = p.pairs + up(static_cast<size_t>(n) * sizeof(int));
+        p.bytes = p.totals;
+    }
+    return p;
+}
+
+size_t SortSmem(int bins) { return ((static_cast<size_t>(kSortWarps) * bins + 1) & ~static_cast<size_t>(1)) * 2 + bins * 4; }
+
+// ---- exchange ----------------------------------------------------------------------------------
+
+// Rows of `bytes` bytes as packs of V: dispatch copies whatever the element type is.  L threads per
+// token, which read a piece of its row once and write it to every choice.
+template <typename V, int L>
+__global__ void __launch_bounds__(kBlock)
+    DispatchKernel(const unsigned char* __restrict__ x, int64_t ldx, int64_t tokens, int packs, int topk,
+                   const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
+                   unsigned char* __restrict__ out, int64_t ldo) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + threadIdx.x / L;
+    if (t >= tokens) return;
+    const int kept = Kept(offsets, experts, pairs);
+    const V* row = reinterpret_cast<const V*>(x + t * ldx);
+    for (int c = threadIdx.x % L; c < packs; c += L) {
+        const V v = row[c];
+        for (int j = 0; j < topk; ++j) {
+            const int p = __ldg(position + t * topk + j);
+            if (static_cast<unsigned>(p) >= static_cast<unsigned>(pairs)) continue;
+            reinterpret_cast<V*>(out + p * ldo)[c] = p < kept ? v : V{};
+        }
+    }
+}
+
+// out[t] = sum over the kept choices of w[t, j] y[position[t, j]], j ascending, in 32 bits.  Rows of
+// dropped choices are never read.  Null weights are ones (the gradient of dispatch).
+template <typename T, int N, int L>
+__global__ void __launch_bounds__(kBlock)
+    CombineKernel(const T* __restrict__ y, int64_t ldy, int64_t tokens, int cols, int topk,
+                  const void* __restrict__ weights, int wtype, const int* __restrict__ position,
+                  const int* __restrict__ offsets, int experts, int pairs, T* __restrict__ out, int64_t ldo) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + threadIdx.x / L;
+    if (t >= tokens) return;
+    const unsigned kept = static_cast<unsigned>(Kept(offsets, experts, pairs));
+    const int full = cols / N;
+    for (int c = threadIdx.x % L; c < full; c += L) {
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+        for (int j = 0; j < topk; ++j) {
+            const unsigned p = static_cast<unsigned>(__ldg(position + t * topk + j));
+            if (p >= kept) continue;
+            const float w = weights ? LoadAs(weights, t * topk + j, wtype) : 1.0f;
+            const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(y + p * ldy + static_cast<int64_t>(c) * N);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = fmaf(w, ToFloat(v.v[i]), acc[i]);
+        }
+        Pack<T, N> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] = FromFloat<T>(acc[i]);
+        *reinterpret_cast<Pack<T, N>*>(out + t * ldo + static_cast<int64_t>(c) * N) = r;
+    }
+    for (int c = full * N + threadIdx.x % L; c < cols; c += L) {
+        float acc = 0.0f;
+        for (int j = 0; j < topk; ++j) {
+            const unsigned p = static_cast<unsigned>(__ldg(position + t * topk + j));
+            if (p >= kept) continue;
+            acc = fmaf(weights ? LoadAs(weights, t * topk + j, wtype) : 1.0f, ToFloat(y[p * ldy + c]), acc);
+        }
+        out[t * ldo + c] = FromFloat<T>(acc);
+    }
+}
+
+// The gradient of combine: dy[position[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], y[position[t, j]]>,
+// zeros where the choice was dropped.  L threads per token; dw's sum over the row goes through
+// registers, then the group's warps in order.
+template <typename T, int N, int L>
+__global__ void __launch_bounds__(kBlock)
+    CombineBackwardKernel(const T* __restrict__ dout, int64_t ldd, const T* __restrict__ y, int64_t ldy, int64_t tokens,
+                          int cols, int topk, const void* __restrict__ weights, int wtype,
+                          const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
+                          T* __restrict__ dy, int64_t lddy, void* __restrict__ dweights) {
+    extern __shared__ float part[];  // [kBlock / 32][topk]
+    const int group = threadIdx.x / L, at = threadIdx.x % L, warp = threadIdx.x >> 5;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + group;
+    const bool real = t < tokens;
+    const int kept = Kept(offsets, experts, pairs);
+    const int full = cols / N;
+    const T* d = dout + (real ? t : 0) * ldd;
+    for (int j = 0; j < topk; ++j) {
+        const int p = real ? __ldg(position + t * topk + j) : -1;
+        float sum = 0.0f;
+        if (p >= 0 && p < kept) {
+            const float w = LoadAs(weights, t * topk + j, wtype);
+            for (int c = at; c < full; c += L) {
+                const Pack<T, N> g = *reinterpret_cast<const Pack<T, N>*>(d + static_cast<int64_t>(c) * N);
+                const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(y + p * ldy + static_cast<int64_t>(c) * N);
+                Pack<T, N> r;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    sum = fmaf(ToFloat(g.v[i]), ToFloat(v.v[i]), sum);
+                    r.v[i] = FromFloat<T>(__fmul_rn(w, ToFloat(g.v[i])));
+                }
+                *reinterpret_cast<Pack<T, N>*>(dy + p * lddy + static_cast<int64_t>(c) * N) = r;
+            }
+            for (int c = full * N + at; c < cols; c += L) {
+                const float g = ToFloat(d[c]);
+                sum = fmaf(g, ToFloat(y[p * ldy + c]), sum);
+                dy[p * lddy + c] = FromFloat<T>(__fmul_rn(w, g));
+            }
+        } else if (p >= 0 && p < pairs) {
+            for (int c = at; c < cols; c += L) dy[p * lddy + c] = FromFloat<T>(0.0f);
+        }
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, o);
+        if ((threadIdx.x & 31) == 0) part[warp * topk + j] = sum;
+    }
+    __syncthreads();
+    if (!real) return;
+    for (int j = at; j < topk; j += L) {
+        float sum = 0.0f;
+        for (int w = 0; w < L / 32; ++w) sum += part[(group * (L / 32) + w) * topk + j];
+        StoreAs(dweights, t * topk + j, wtype, sum);
+    }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+
+bool IsFloat(int dtype) { return dtype == STLQ_B200_F32 || dtype == STLQ_B200_BF16 || dtype == STLQ_B200_F16; }
+int64_t SizeOf(int dtype) { return dtype == STLQ_B200_F32 ? 4 : 2; }
+bool Aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(to) == 0; }
+int Bad(const char* msg) { return SetError(STLQ_B200_EINVAL, msg); }
+
+template <typename F>
+int Guard(F&& f) {
+    try {
+        return f();
+    } catch (...) {
+        return STLQ_B200_ENOMEM;  // the only thing that throws here is a message's memory
+    }
+}
+
+template <typename F>
+void ForType(int dtype, F&& f) {
+    if (dtype == STLQ_B200_F32) f(float{});
+    else if (dtype == STLQ_B200_BF16) f(__nv_bfloat16{});
+    else f(__half{});
+}
+
+// Threads per row: enough that a thread has at most four packs of it, a warp for short rows.
+template <typename F>
+void ForLanes(int64_t packs, F&& f) {
+    if (packs <= 128) f(std::integral_constant<int, 32>{});
+    else if (packs <= 512) f(std::integral_constant<int, 128>{});
+    else f(std::integral_constant<int, 256>{});
+}
+
+// Blocks for `rows` rows at L threads each; 0 if they do not fit a grid.
+unsigned Blocks(int64_t rows, int L) {
+    const int64_t b = (rows + kBlock / L - 1) / (kBlock / L);
+    return b > 0x7fffffff ? 0u : static_cast<unsigned>(b);
+}
+
+int CheckRouting(int64_t tokens, int topk, int experts, const void* position, const void* offsets) {
+    if (tokens < 0 || topk < 1 || topk > STLQ_B200_MAX_TOPK) return Bad("tokens >= 0 and 1 <= topk <= 64 required");
+    if (experts < 1 || experts > STLQ_B200_MAX_ROOT) return Bad("1 <= experts <= 65536 required");
+    if (tokens > 0x7fffffff / topk) return Bad("tokens * topk must be below 2^31");
+    if (tokens > 0 && (!position || !offsets)) return Bad("null position or offsets");
+    if (!Aligned(position, 4) || !Aligned(offsets, 4)) return Bad("position and offsets must be 4-byte aligned");
+    return 0;
+}
+
+int Quantize(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int64_t rows, int cols, int topk,
+             const int* position, const int* offsets, int experts, int8_t* q, int64_t ldq, float* scale, void* stream) {
+    if (!IsFloat(x_dtype)) return Bad("x_dtype must be F32, BF16 or F16");
+    if (rows < 0 || cols < 0) return Bad("rows and cols must be >= 0");
+    if (ldx < cols || ldq < cols) return Bad("ldx or ldq below cols");
+    if (rows == 0) return 0;
+    if (!scale || (cols > 0 && (!x || !q))) return Bad("null pointer");
+    if (!Aligned(x, SizeOf(x_dtype)) || !Aligned(scale, 4)) return Bad("x or scale not aligned to its element");
+    DeviceScope scope(k->device);
+    if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int pairs = position ? static_cast<int>(rows * topk) : 0;
+    bool fits = true;
+    ForType(x_dtype, [&](auto one) {
+        using T = decltype(one);
+        constexpr int N = 16 / sizeof(T);
+        const T* xp = static_cast<const T*>(x);
+        const bool wide = Aligned(x, 16) && ldx % N == 0 && Aligned(q, N) && ldq % N == 0;
+        ForLanes(wide ? cols / N : cols, [&](auto lanes) {
+            constexpr int L = decltype(lanes)::value;
+            const unsigned grid = Blocks(rows, L);
+            fits = grid != 0;
+            if (!fits) return;
+            if (wide)
+                QuantizeRowsKernel<T, N, L><<<grid, kBlock, 0, s>>>(xp, ldx, rows, cols, topk, position, offsets, experts,
+                                                                    pairs, q, ldq, scale);
+            else
+                QuantizeRowsKernel<T, 1, L><<<grid, kBlock, 0, s>>>(xp, ldx, rows, cols, topk, position, offsets, experts,
+                                                                    pairs, q, ldq, scale);
+        });
+    });
+    if (!fits) return Bad("too many rows");
+    return Ck(cudaGetLastError(), "quantize_rows");
+}
+
+}  // namespace
+
+extern "C" {
+
+int stlq_b200_quantize_rows(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int64_t rows, int cols,
+                            int8_t* q, int64_t ldq, float* scale, void* stream) {
+    return Guard([&] {
+        if (!k) return Bad("kernel-provider handle is null");
+        return Quantize(k, x, x_dtype, ldx, rows, cols, 1, nullptr, nullptr, 0, q, ldq, scale, stream);
+    });
+}
+
+int stlq_b200_dispatch_i8(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int64_t tokens, int cols, int topk,
+                          const int32_t* position, const int32_t* offsets, int experts, int8_t* q, int64_t ldq,
+                          float* scale, void* stream) {
+    return Guard([&] {
+        if (!k) return Bad("kernel-provider handle is null");
+        if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
+        return Quantize(k, x, x_dtype, ldx, tokens, cols, topk, position, offsets, experts, q, ldq, scale, stream);
+    });
+}
+
+int stlq_b200_sort_by_expert_workspace(int64_t tokens, int topk, int experts, size_t* bytes) {
+    return Guard([&] {
+        if (!bytes) return Bad("bytes is null");
+        *bytes = 0;
+        if (int rc = CheckRouting(tokens, topk, experts, bytes, bytes)) return rc;
+        *bytes = PlanSort(tokens * topk, experts).bytes;
+        return 0;
+    });
+}
+
+int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtype, int64_t tokens, int topk, int experts,
+                             int32_t* order, int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+    return Guard([&] {
+        if (!k) return Bad("kernel-provider handle is null");
+        if (ids_dtype != STLQ_B200_I32 && ids_dtype != STLQ_B200_I64) return Bad("ids_dtype must be I32 or I64");
+        if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
+        if (!offsets) return Bad("null offsets");
+        const int n = static_cast<int>(tokens * topk);
+        if (n > 0 && (!ids || !order)) return Bad("null ids or order");
+        if (!Aligned(ids, ids_dtype == STLQ_B200_I64 ? 8 : 4) || !Aligned(order, 4)) return Bad("ids or order not aligned to its element");
+        const SortPlan p = PlanSort(n, experts);
+        if (workspace_bytes < p.bytes || (p.bytes && (!workspace || !Aligned(workspace, 16))))
+            return Bad("workspace below stlq_b200_sort_by_expert_workspace's bytes, or not 16-byte aligned");
+        DeviceScope scope(k->device);
+        if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (n == 0) {
+            NoPairsKernel<<<std::min(experts / 256 + 1, 64), 256, 0, s>>>(offsets, experts + 1);
+            return Ck(cudaGetLastError(), "sort_by_expert");
+        }
+        char* ws = static_cast<char*>(workspace);
+        int* hist = reinterpret_cast<int*>(ws);
+        int* keys = reinterpret_cast<int*>(ws + p.keys);
+        int* pairs = reinterpret_cast<int*>(ws + p.pairs);
+        if (int rc = Ck(cudaFuncSetAttribute(SortScatterKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10), "sort_by_expert")) return rc;
+        if (int rc = Ck(cudaFuncSetAttribute(SortCountKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10), "sort_by_expert")) return rc;
+        SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, nullptr, n, experts, 0, 0x7fffffff, p.bins[0], p.tiles};
+        if (p.passes == 1) {
+            SortCountKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, nullptr);
+            SortScanKernel<<<1, 1024, 0, s>>>(hist, static_cast<int64_t>(a.bins) * p.tiles, nullptr, 0);
+            SortScatterKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, nullptr, order, position, offsets);
+            return Ck(cudaGetLastError(), "sort_by_expert");
+        }
+        if (int rc = Ck(cudaMemsetAsync(offsets, 0, sizeof(int) * (static_cast<size_t>(experts) + 1), s), "sort_by_expert")) return rc;
+        a.mask = p.bins[0] - 1;
+        SortCountKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, offsets);
+        SortScanKernel<<<2, 1024, 0, s>>>(hist, static_cast<int64_t>(a.bins) * p.tiles, offsets, experts + 1);
+        SortScatterKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, keys, pairs, nullptr, nullptr);
+        SortPass b{nullptr, 0, keys, pairs, n, experts, p.shift[1], 0x7fffffff, p.bins[1], p.tiles};
+        SortCountKernel<<<p.tiles, kSortBlock, SortSmem(b.bins), s>>>(b, hist, nullptr);
+        SortScanKernel<<<1, 1024, 0, s>>>(hist, static_cast<int64_t>(b.bins) * p.tiles, nullptr, 0);
+        SortScatterKernel<<<p.tiles, kSortBlock, SortSmem(b.bins), s>>>(b, hist, nullptr, order, position, nullptr);
+        return Ck(cudaGetLastError(), "sort_by_expert");
+    });
+}
+
+int stlq_b200_dispatch(stlq_b200_kernels* k, const void* x, int elem_bytes, int64_t ldx, int64_t tokens, int cols, int topk,
+                       const int32_t* position, const int32_t* offsets, int experts, void* out, int64_t ldo, void* stream) {
+    return Guard([&] {
+        if (!k) return Bad("kernel-provider handle is null");
+        if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return Bad("elem_bytes must be 1, 2 or 4");
+        if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
+        if (cols < 0 || ldx < cols || ldo < cols) return Bad("cols >= 0, ldx >= cols and ldo >= cols required");
+        if (tokens == 0 || cols == 0) return 0;
+        if (!x || !out) return Bad("null x or out");
+        if (!Aligned(x, elem_bytes) || !Aligned(out, elem_bytes)) return Bad("x or out not aligned to its element");
+        if (cols > 0x7fffffff / elem_bytes) return Bad("rows of 2^31 bytes or more");
+        DeviceScope scope(k->device);
+        if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const int pairs = static_cast<int>(tokens * topk);
+        const int bytes = cols * elem_bytes;
+        const int64_t bx = ldx * elem_bytes, bo = ldo * elem_bytes;
+        bool fits = true;
+        auto launch = [&](auto pack) {
+            using V = decltype(pack);
+            const int packs = bytes / static_cast<int>(sizeof(V));
+            ForLanes(packs, [&](auto lanes) {
+                constexpr int L = decltype(lanes)::value;
+                const unsigned grid = Blocks(tokens, L);
+                fits = grid != 0;
+                if (!fits) return;
+                DispatchKernel<V, L><<<grid, kBlock, 0, s>>>(static_cast<const unsigned char*>(x), bx, tokens, packs, topk,
+                                                             position, offsets, experts, pairs,
+                                                             static_cast<unsigned char*>(out), bo);
+            });
+        };
+        // The widest access that the rows, their strides and both bases allow.
+        auto fit = [&](int v) { return bytes % v == 0 && bx % v == 0 && bo % v == 0 && Aligned(x, v) && Aligned(out, v); };
+        if (fit(16)) launch(uint4{});
+        else if (fit(8)) launch(uint2{});
+        else if (fit(4)) launch(uint32_t{});
+        else if (fit(2)) launch(uint16_t{});
+        else launch(uint8_t{});
+        if (!fits) return Bad("too many tokens");
+        return Ck(cudaGetLastError(), "dispatch");
+    });
+}
+
+int stlq_b200_combine(stlq_b200_kernels* k, const void* y, int dtype, int64_t ldy, int64_t tokens, int cols, int topk,
+                      const void* weights, int weights_dtype, const int32_t* position, const int32_t* offsets, int experts,
+                      void* out, int64_t ldo, void* stream) {
+    return Guard([&] {
+        if (!k) return Bad("kernel-provider handle is null");
+        if (!IsFloat(dtype) || (weights && !IsFloat(weights_dtype))) return Bad("dtypes must be F32, BF16 or F16");
+        if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
+        if (cols < 0 || ldy < cols || ldo < cols) return Bad("cols >= 0, ldy >= cols and ldo >= cols required");
+        if (tokens == 0 || cols == 0) return 0;
+        if (!y || !out) return Bad("null y or out");
+        if (!Aligned(y, SizeOf(dtype)) || !Aligned(out, SizeOf(dtype)) || (weights && !Aligned(weights, SizeOf(weights_dtype))))
+            return Bad("y, weights or out not aligned to its element");
+        DeviceScope scope(k->device);
+        if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const int pairs = static_cast<int>(tokens * topk);
+        bool fits = true;
+        ForType(dtype, [&](auto one) {
+            using T = decltype(one);
+            constexpr int N = 16 / sizeof(T);
+            const bool wide = Aligned(y, 16) && ldy % N == 0 && Aligned(out, 16) && ldo % N == 0;
+            ForLanes(wide ? cols / N : cols, [&](auto lanes) {
+                constexpr int L = decltype(lanes)::value;
+                const unsigned grid = Blocks(tokens, L);
+                fits = grid != 0;
+                if (!fits) return;
+                const T* yp = static_cast<const T*>(y);
+                T* op = static_cast<T*>(out);
+                if (wide)
+                    CombineKernel<T, N, L><<<grid, kBlock, 0, s>>>(yp, ldy, tokens, cols, topk, weights, weights_dtype,
+                                                                   position, offsets, experts, pairs, op, ldo);
+                else
+                    CombineKernel<T, 1, L><<<grid, kBlock, 0, s>>>(yp, ldy, tokens, cols, topk, weights, weights_dtype,
+                                                                   position, offsets, experts, pairs, op, ldo);
+            });
+        });
+        if (!fits) return Bad("too many tokens");
+        return Ck(cudaGetLastError(), "combine");
+    });
+}
+
+int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype, int64_t ldd, const void* y, int64_t ldy,
+                               int64_t tokens, int cols, int topk, const void* weights, int weights_dtype,
+                               const int32_t* position, const int32_t* offsets, int experts, void* dy, int64_t lddy,
+                               void* dweights, void* stream) {
+    return Guard([&] {
+        if (!k) return Bad("kernel-provider handle is null");
+        if (!IsFloat(dtype) || !IsFloat(weights_dtype)) return Bad("dtypes must be F32, BF16 or F16");
+        if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
+        if (cols < 0 || ldd < cols || ldy < cols || lddy < cols) return Bad("cols >= 0 and leading dimensions >= cols required");
+        if (tokens == 0) return 0;
+        if (!weights || !dweights || (cols > 0 && (!dout || !y || !dy))) return Bad("null pointer");
+        if (!Aligned(dout, SizeOf(dtype)) || !Aligned(y, SizeOf(dtype)) || !Aligned(dy, SizeOf(dtype)) ||
+            !Aligned(weights, SizeOf(weights_dtype)) || !Aligned(dweights, SizeOf(weights_dtype)))
+            return Bad("a pointer is not aligned to its element");
+        DeviceScope scope(k->device);
+        if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const int pairs = static_cast<int>(tokens * topk);
+        const size_t smem = sizeof(float) * (kBlock / 32) * topk;
+        bool fits = true;
+        ForType(dtype, [&](auto one) {
+            using T = decltype(one);
+            constexpr int N = 16 / sizeof(T);
+            const bool wide = Aligned(dout, 16) && ldd % N == 0 && Aligned(y, 16) && ldy % N == 0 && Aligned(dy, 16) && lddy % N == 0;
+            ForLanes(wide ? cols / N : cols, [&](auto lanes) {
+                constexpr int L = decltype(lanes)::value;
+                const unsigned grid = Blocks(tokens, L);
+                fits = grid != 0;
+                if (!fits) return;
+                const T *dp = static_cast<const T*>(dout), *yp = static_cast<const T*>(y);
+                T* op = static_cast<T*>(dy);
+                if (wide)
+                    CombineBackwardKernel<T, N, L><<<grid, kBlock, smem, s>>>(dp, ldd, yp, ldy, tokens, cols, topk, weights,
+                                                                              weights_dtype, position, offsets, experts,
+                                                                              pairs, op, lddy, dweights);
+                else
+                    CombineBackwardKernel<T, 1, L><<<grid, kBlock, smem, s>>>(dp, ldd, yp, ldy, tokens, cols, topk, weights,
+                                                                              weights_dtype, position, offsets, experts,
+                                                                              pairs, op, lddy, dweights);
+            });
+        });
+        if (!fits) return Bad("too many tokens");
+        return Ck(cudaGetLastError(), "combine_backward");
+    });
+}
+
+}  // extern "C"
