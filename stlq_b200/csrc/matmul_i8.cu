@@ -26,20 +26,29 @@ using stlq_b200::DeviceScope;
 using stlq_b200::SetError;
 namespace tc = stlq_b200::tc;
 
-constexpr int kChannels = 128;                       // channels of a tile (the MMA's M)
+constexpr int kChannels = 128;                       // channels of a CTA's tile (its share of the MMA's M)
 constexpr int kTileK = 128;                          // bytes of a 128-byte swizzle row
 constexpr uint32_t kWBytes = kChannels * kTileK;
-constexpr int kThreads = 192;                        // warp 0 loads, warp 1 multiplies, 2..5 write
+constexpr int kWriters = 8;                          // warps of the epilogue, two for each quarter of the TMEM lanes
+constexpr int kThreads = 64 + 32 * kWriters;         // warp 0 loads, warp 1 multiplies, the others write
 constexpr uint64_t kWaitNs = 2000000000ull;          // 2 s per barrier wait
 constexpr int kBand = 8;                             // row tiles that run side by side over the channels
 
-template <int kRows>
+// kOne: a CTA computes tiles of its own, one after the other.  kPair: two CTAs share a tile of 256
+// channels (tcgen05 cta_group::2): each holds its channels and half of the rows, so that an operand
+// byte in shared memory is used twice as often.  kSplit: the CTAs of a cluster each sum a part of kdim
+// for one tile and add up over distributed shared memory, for products with few tiles.
+enum Mode { kOne, kPair, kSplit };
+
+template <int kRows, Mode kMode>
 struct Shape {
-    static constexpr uint32_t kXBytes = kRows * kTileK;
+    static constexpr uint32_t kXBytes = (kMode == kPair ? kRows / 2 : kRows) * kTileK;
     static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
     static constexpr int kStages = std::min<int>(10, 200 * 1024 / kStageBytes);
-    static constexpr int kColumns = kRows < 32 ? 32 : kRows;  // TMEM columns of one accumulator
-    static constexpr uint32_t kTmem = 2 * kColumns;           // two: one is written out while the next is made
+    static constexpr int kColumns = kRows < 32 ? 32 : kRows;        // TMEM columns of one accumulator
+    static constexpr uint32_t kTmem = (kMode == kSplit ? 1 : 2) * kColumns;  // two: one is written out while the next is made
+    static constexpr int kTileChannels = kMode == kPair ? 2 * kChannels : kChannels;
+    static constexpr int kGranule = kMode == kPair ? 32 : 16;       // rows of an MMA come in multiples of this
 };
 
 struct MatmulArgs {
@@ -74,10 +83,10 @@ struct Segments {
     int* end;
 };
 
-template <int kRows>
+template <int kRows, int kTileChannels>
 __device__ __forceinline__ Tile FindTile(const MatmulArgs& a, const Segments& sg, int id) {
     Tile t;
-    const int ct = (a.n + kChannels - 1) / kChannels;
+    const int ct = (a.n + kTileChannels - 1) / kTileChannels;
     int local = id;
     if (a.offsets) {
         int lo = 0, hi = a.experts;  // the last expert whose tiles begin at or before id
@@ -100,15 +109,16 @@ __device__ __forceinline__ Tile FindTile(const MatmulArgs& a, const Segments& sg
     const int rt = (t.end - t.row0 + kRows - 1) / kRows;
     const int band = local / (kBand * ct), in = local - band * kBand * ct;
     const int height = min(kBand, rt - band * kBand);
-    t.channel0 = in / height * kChannels;
+    t.channel0 = in / height * kTileChannels;
     t.row0 += (band * kBand + in % height) * kRows;
     return t;
 }
 
-template <int kRows, typename T>
+template <int kRows, Mode kMode, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
-    MatmulI8Kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const MatmulArgs a) {
-    using S = Shape<kRows>;
+    MatmulI8Kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const MatmulArgs a,
+                   int cluster) {
+    using S = Shape<kRows, kMode>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = smem_raw + ((1024 - (tc::SmemAddr(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(base + S::kStages * S::kStageBytes);
@@ -116,14 +126,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* made = empty + S::kStages;  // an accumulator is complete
     uint64_t* taken = made + 2;           // an accumulator has been read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
+    float* row_scales = reinterpret_cast<float*>(tmem_slot + 4);  // [kWriters][kRows]
     Segments sg;
-    sg.first = reinterpret_cast<int*>(tmem_slot + 4);
+    sg.first = reinterpret_cast<int*>(row_scales + kWriters * kRows);
     sg.begin = sg.first + (a.experts + 1);
     sg.end = sg.begin + a.experts;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int ct = (a.n + kChannels - 1) / kChannels;
+    const int rank = kMode == kOne ? 0 : static_cast<int>(tc::ClusterRank());
+    const int ct = (a.n + S::kTileChannels - 1) / S::kTileChannels;
     const int nk = (a.kdim + kTileK - 1) / kTileK;
+    // The steps of kdim that this CTA sums (all, but for kSplit).
+    const int k_first = kMode == kSplit ? static_cast<int>(static_cast<int64_t>(nk) * rank / cluster) : 0;
+    const int k_last = kMode == kSplit ? static_cast<int>(static_cast<int64_t>(nk) * (rank + 1) / cluster) : nk;
+    const int first_tile = kMode == kOne ? blockIdx.x : blockIdx.x / cluster;
+    const int tile_step = kMode == kOne ? gridDim.x : gridDim.x / cluster;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -132,11 +149,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             tc::MbarInit(&made[b], 1);
-            tc::MbarInit(&taken[b], 4);
+            tc::MbarInit(&taken[b], kMode == kPair ? 2 * kWriters : kWriters);
         }
         tc::FenceBarrierInit();
     }
-    if (warp == 1) tc::TmemAlloc(tmem_slot, S::kTmem);
+    if (warp == 1) {
+        if constexpr (kMode == kPair) tc::TmemAllocPair(tmem_slot, S::kTmem);
+        else tc::TmemAlloc(tmem_slot, S::kTmem);
+    }
     if (a.offsets) {
         for (int e = threadIdx.x; e < a.experts; e += kThreads) sg.end[e] = min(max(a.offsets[e + 1], 0), a.rows);
         __syncthreads();
@@ -172,98 +192,189 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     tc::FenceBeforeSync();
-    __syncthreads();
+    if constexpr (kMode == kPair) {
+        __syncthreads();
+        tc::ClusterSync();  // the pair's barriers exist before either arrives on them
+    } else {
+        __syncthreads();
+    }
     tc::FenceAfterSync();
     const uint32_t tmem = *tmem_slot;
     const int tiles = a.offsets ? sg.first[a.experts] : (a.rows + kRows - 1) / kRows * ct;
+    // Rows of a tile's MMA: what is left of the segment, rounded up.
+    auto columns = [](const Tile& t) { return min(kRows, (t.end - t.row0 + S::kGranule - 1) / S::kGranule * S::kGranule); };
 
     if (warp == 0 && lane == 0) {
-        int64_t step = 0;
+        int step = 0;
         bool ok = true;
-        for (int id = blockIdx.x; id < tiles && ok; id += gridDim.x) {
-            const Tile t = FindTile<kRows>(a, sg, id);
-            const int wrow = t.expert * a.n + t.channel0;
-            for (int kb = 0; kb < nk; ++kb, ++step) {
-                const int s = static_cast<int>(step % S::kStages);
-                const int64_t round = step / S::kStages;
+        for (int id = first_tile; id < tiles && ok; id += tile_step) {
+            const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
+            const int wrow = t.expert * a.n + t.channel0 + (kMode == kPair ? rank * kChannels : 0);
+            const int xrow = t.row0 + (kMode == kPair ? rank * (columns(t) / 2) : 0);
+            for (int kb = k_first; kb < k_last; ++kb, ++step) {
+                const int s = step % S::kStages, round = step / S::kStages;
                 if (round > 0 && !(ok = tc::MbarWait(&empty[s], (round - 1) & 1, a.err, kWaitNs))) break;
                 unsigned char* st = base + s * S::kStageBytes;
-                tc::MbarArriveExpectTx(&full[s], S::kStageBytes);
-                tc::TmaLoad2d(st, &tw, &full[s], kb * kTileK, wrow);
-                tc::TmaLoad2d(st + kWBytes, &tx, &full[s], kb * kTileK, t.row0);
+                if constexpr (kMode == kPair) {
+                    // The even CTA's barrier counts the bytes of both.
+                    if (rank == 0) tc::MbarArriveExpectTx(&full[s], 2 * S::kStageBytes);
+                    const uint32_t bar = tc::ClusterAddr(&full[s], 0);
+                    tc::TmaLoad2dPair(st, &tw, bar, kb * kTileK, wrow);
+                    tc::TmaLoad2dPair(st + kWBytes, &tx, bar, kb * kTileK, xrow);
+                } else {
+                    tc::MbarArriveExpectTx(&full[s], S::kStageBytes);
+                    tc::TmaLoad2d(st, &tw, &full[s], kb * kTileK, wrow);
+                    tc::TmaLoad2d(st + kWBytes, &tx, &full[s], kb * kTileK, xrow);
+                }
             }
         }
         // Copies still in flight land before the block may exit.
-        for (int64_t i = step - 1; i >= 0 && i >= step - S::kStages; --i)
-            tc::MbarWait(&full[i % S::kStages], (i / S::kStages) & 1, a.err, kWaitNs, false);
-    } else if (warp == 1 && lane == 0) {
-        constexpr uint32_t idesc = tc::InstrDescI8(kChannels, kRows);
-        int64_t step = 0;
-        int done = 0;
+        if (kMode != kPair || rank == 0)
+            for (int i = step - 1; i >= 0 && i >= step - S::kStages; --i)
+                tc::MbarWait(&full[i % S::kStages], (i / S::kStages) & 1, a.err, kWaitNs, false);
+        if (kMode == kPair && !ok) {  // the other CTA's barrier says no more: leave them 10 ms
+            const uint64_t t0 = tc::GlobalTimerNs();
+            while (tc::GlobalTimerNs() - t0 < 10000000ull) {
+            }
+        }
+    } else if (warp == 1 && lane == 0 && (kMode != kPair || rank == 0)) {
+        int step = 0, done = 0;
         bool ok = true;
-        for (int id = blockIdx.x; id < tiles && ok; id += gridDim.x, ++done) {
-            const int b = done & 1, use = done >> 1;
+        for (int id = first_tile; id < tiles && ok; id += tile_step, ++done) {
+            const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
+            const uint32_t idesc = tc::InstrDescI8(S::kTileChannels, columns(t));
+            const int b = kMode == kSplit ? 0 : done & 1, use = done >> 1;
             if (use > 0 && !(ok = tc::MbarWait(&taken[b], (use - 1) & 1, a.err, kWaitNs))) break;
             tc::FenceAfterSync();
-            for (int kb = 0; kb < nk; ++kb, ++step) {
-                const int s = static_cast<int>(step % S::kStages);
+            for (int kb = k_first; kb < k_last; ++kb, ++step) {
+                const int s = step % S::kStages;
                 if (!(ok = tc::MbarWait(&full[s], (step / S::kStages) & 1, a.err, kWaitNs))) break;
                 tc::FenceAfterSync();
                 const uint32_t w = tc::SmemAddr(base + s * S::kStageBytes), x = w + kWBytes;
 #pragma unroll
-                for (int k = 0; k < kTileK / 32; ++k)
-                    tc::UmmaI8(tmem + b * S::kColumns, tc::SmemDescSw128(w + k * 32), tc::SmemDescSw128(x + k * 32), idesc,
-                               (kb > 0 || k > 0) ? 1u : 0u);
-                tc::UmmaCommit(&empty[s]);
+                for (int k = 0; k < kTileK / 32; ++k) {
+                    const uint64_t dw = tc::SmemDescSw128(w + k * 32), dx = tc::SmemDescSw128(x + k * 32);
+                    const uint32_t more = (kb > k_first || k > 0) ? 1u : 0u;
+                    if constexpr (kMode == kPair) tc::UmmaI8Pair(tmem + b * S::kColumns, dw, dx, idesc, more);
+                    else tc::UmmaI8(tmem + b * S::kColumns, dw, dx, idesc, more);
+                }
+                if constexpr (kMode == kPair) tc::UmmaCommitPair(&empty[s]);
+                else tc::UmmaCommit(&empty[s]);
             }
-            if (ok) tc::UmmaCommit(&made[b]);
+            if (ok) {
+                if constexpr (kMode == kPair) tc::UmmaCommitPair(&made[b]);
+                else tc::UmmaCommit(&made[b]);
+            }
         }
     } else if (warp >= 2) {
         const int quarter = warp & 3;  // the TMEM lanes this warp may read
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const int half = (warp - 2) >> 2;  // its 16 columns of every 32
+        float* scales = row_scales + (warp - 2) * kRows;
+        int* parts = reinterpret_cast<int*>(base);  // kSplit: [kRows][kChannels] over the stages, once they are read
         T* out = static_cast<T*>(a.out);
         int done = 0;
         bool ok = true;
-        for (int id = blockIdx.x; id < tiles && ok; id += gridDim.x, ++done) {
-            const Tile t = FindTile<kRows>(a, sg, id);
-            const int b = done & 1;
-            const int c = t.channel0 + quarter * 32 + lane;
+        for (int id = first_tile; id < tiles && ok; id += tile_step, ++done) {
+            const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
+            const int b = kMode == kSplit ? 0 : done & 1;
+            const int c = t.channel0 + (kMode == kPair ? rank * kChannels : 0) + quarter * 32 + lane;
             const bool real = c < a.n;
             const int64_t wc = static_cast<int64_t>(t.expert) * a.n + c;
             const float ws = real ? a.w_scale[wc] : 0.0f;
             const float bias = real && a.bias ? a.bias[wc] : 0.0f;
-            ok = __all_sync(0xffffffffu, tc::MbarWait(&made[b], (done >> 1) & 1, a.err, kWaitNs));
-            if (!ok) break;
-            tc::FenceAfterSync();
-#pragma unroll 1
-            for (int c0 = 0; c0 < kRows; c0 += 16) {
-                const int r0 = t.row0 + c0;
-                if (r0 >= t.end) break;
-                int v[16];
-                tc::TmemLoad16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * S::kColumns + c0, v);
-                const float qs = r0 + (lane & 15) < t.end ? a.q_scale[r0 + (lane & 15)] : 0.0f;
-                tc::TmemLoadWait();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float s = __shfl_sync(0xffffffffu, qs, j);
-                    const float y = fmaf(__int2float_rn(v[j]) * s, ws, bias);
-                    if (real && r0 + j < t.end) out[(static_cast<int64_t>(r0) + j) * a.ldo + c] = Out<T>(y);
-                }
-            }
-            tc::FenceBeforeSync();
+            const int count = min(kRows, t.end - t.row0);
+            for (int r = lane; r < count; r += 32) scales[r] = a.q_scale[t.row0 + r];
             __syncwarp();
-            if (lane == 0) tc::MbarArrive(&taken[b]);
-        }
-        // Rows after the last segment (dropped choices) hold zeros.
-        if (a.offsets) {
-            const int64_t kept = sg.end[a.experts - 1];
-            const int64_t left = (a.rows - kept) * a.n;
-            for (int64_t i = blockIdx.x * 128 + threadIdx.x - 64; i < left; i += gridDim.x * 128)
-                out[(kept + i / a.n) * a.ldo + i % a.n] = Out<T>(0.0f);
+            T* to = out + (static_cast<int64_t>(t.row0) + half * 16) * a.ldo + c;
+            ok = __all_sync(0xffffffffu, tc::MbarWait(&made[b], (done >> 1) & 1, a.err, kWaitNs));
+            if (ok) {
+                tc::FenceAfterSync();
+                const uint32_t from = tmem + lanes + b * S::kColumns;
+                auto write = [&](const int (&v)[16], int c0) {
+                    if constexpr (kMode == kSplit) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) parts[(c0 + j) * kChannels + quarter * 32 + lane] = v[j];
+                    } else {
+                        float y[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j] = fmaf(__int2float_rn(v[j]) * scales[c0 + j], ws, bias);
+                        const int left = real ? count - c0 : 0;
+                        T* row = to;
+                        if (left >= 16) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j, row += a.ldo) *row = Out<T>(y[j]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j, row += a.ldo)
+                                if (j < left) *row = Out<T>(y[j]);
+                        }
+                        to += 32 * a.ldo;
+                    }
+                };
+                // The next 16 columns are on their way while 16 are written.
+                int va[16], vb[16];
+                int c0 = half * 16;
+                if (c0 < count) tc::TmemLoad16(from + c0, va);
+#pragma unroll 1
+                for (; c0 < count; c0 += 64) {
+                    tc::TmemLoadWait(va);
+                    if (c0 + 32 < count) tc::TmemLoad16(from + c0 + 32, vb);
+                    write(va, c0);
+                    if (c0 + 32 >= count) break;
+                    tc::TmemLoadWait(vb);
+                    if (c0 + 64 < count) tc::TmemLoad16(from + c0 + 64, va);
+                    write(vb, c0 + 32);
+                }
+                tc::FenceBeforeSync();
+            }
+            __syncwarp();
+            if constexpr (kMode == kSplit) break;  // one tile each; its rows are finished below
+            if (ok && lane == 0) {
+                if (kMode == kPair && rank != 0) tc::MbarArriveCluster(tc::ClusterAddr(&taken[b], 0));
+                else tc::MbarArrive(&taken[b]);
+            }
         }
     }
+    if constexpr (kMode == kSplit) {
+        // Row j of the tile is finished by CTA j % cluster: the parts in order of kdim.  A quarter's two
+        // warps take these rows in turn.
+        tc::FenceBeforeSync();
+        __syncwarp();
+        tc::ClusterSync();
+        if (warp >= 2 && first_tile < tiles) {
+            const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, first_tile);
+            const int at = (warp & 3) * 32 + lane, c = t.channel0 + at;
+            const int64_t wc = static_cast<int64_t>(t.expert) * a.n + c;
+            const int count = min(kRows, t.end - t.row0);
+            if (c < a.n) {
+                const float ws = a.w_scale[wc], bias = a.bias ? a.bias[wc] : 0.0f;
+                const float* scales = row_scales + (warp - 2) * kRows;
+                for (int j = rank + cluster * ((warp - 2) >> 2); j < count; j += 2 * cluster) {
+                    int sum = 0;
+#pragma unroll 8
+                    for (int r = 0; r < cluster; ++r) sum += tc::LoadCluster(tc::ClusterAddr(base, r) + (j * kChannels + at) * 4);
+                    static_cast<T*>(a.out)[(static_cast<int64_t>(t.row0) + j) * a.ldo + c] =
+                        Out<T>(fmaf(__int2float_rn(sum) * scales[j], ws, bias));
+                }
+            }
+        }
+    }
+    if (a.offsets && warp >= 2) {  // rows after the last segment (dropped choices) hold zeros
+        T* out = static_cast<T*>(a.out);
+        const int64_t kept = sg.end[a.experts - 1];
+        const int64_t left = (a.rows - kept) * a.n;
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * (32 * kWriters) + threadIdx.x - 64; i < left; i += gridDim.x * (32 * kWriters))
+            out[(kept + i / a.n) * a.ldo + i % a.n] = Out<T>(0.0f);
+    }
     tc::FenceBeforeSync();
-    __syncthreads();
-    if (warp == 1) tc::TmemDealloc(tmem, S::kTmem);
+    __syncwarp();
+    if constexpr (kMode == kOne) __syncthreads();
+    else tc::ClusterSync();  // no CTA leaves while another reads its memory or arrives on its barriers
+    if (warp == 1) {
+        if constexpr (kMode == kPair) tc::TmemDeallocPair(tmem, S::kTmem);
+        else tc::TmemDealloc(tmem, S::kTmem);
+    }
 }
 
 // Without a term to sum (kdim 0): the bias, and zeros after the last segment.
@@ -317,38 +428,76 @@ bool MakeMap(CUtensorMap* map, const int8_t* p, int64_t rows, int kdim, int64_t 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kRows, typename T>
-cudaError_t LaunchRows(const CUtensorMap& tw, const int8_t* q, int64_t ldq, const MatmulArgs& a, int sms, cudaStream_t s) {
-    using S = Shape<kRows>;
-    CUtensorMap tx;
-    if (!MakeMap(&tx, q, a.rows, a.kdim, ldq, kRows)) return cudaErrorInvalidValue;
-    const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + (2 * S::kStages + 4) * 8 + 16 +
-                        (a.offsets ? (3 * static_cast<size_t>(a.experts) + 1) * 4 : 0);
-    const auto kernel = MatmulI8Kernel<kRows, T>;
-    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); e != cudaSuccess) return e;
-    const int64_t ct = (a.n + kChannels - 1) / kChannels;
-    const int64_t most = (static_cast<int64_t>(a.rows) + kRows - 1) / kRows + (a.offsets ? a.experts : 0);
-    const int grid = static_cast<int>(std::min<int64_t>(sms, ct * most));
-    kernel<<<grid, kThreads, smem, s>>>(tw, tx, a);
-    return cudaGetLastError();
+struct Operands {
+    const int8_t* q;
+    int64_t ldq;
+    const int8_t* w;
+    int64_t ldw;
+    int sms;
+    cudaStream_t stream;
+};
+
+// The most row tiles that `rows` rows in `experts` segments can make.
+int64_t MostRowTiles(const MatmulArgs& a, int height) {
+    const int64_t full = (static_cast<int64_t>(a.rows) + height - 1) / height;
+    return a.offsets ? std::min<int64_t>(a.rows, full + a.experts) : full;
 }
 
-// The tile's width in rows: the least that holds a segment (their mean, for experts), so that few
-// rows cost few columns; wider tiles read a weight fewer times.
+template <int kRows, Mode kMode, typename T>
+cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
+    using S = Shape<kRows, kMode>;
+    CUtensorMap tw, tx;
+    if (!MakeMap(&tw, o.w, static_cast<int64_t>(a.experts) * a.n, a.kdim, o.ldw, kChannels) ||
+        !MakeMap(&tx, o.q, a.rows, a.kdim, o.ldq, kMode == kPair ? kRows / 2 : kRows))
+        return cudaErrorInvalidValue;
+    const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + (2 * S::kStages + 4) * 8 + 16 + 4 * kWriters * kRows +
+                        (a.offsets ? (3 * static_cast<size_t>(a.experts) + 1) * 4 : 0);
+    const auto kernel = MatmulI8Kernel<kRows, kMode, T>;
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); e != cudaSuccess) return e;
+    const int64_t tiles = MostRowTiles(a, kRows) * ((a.n + S::kTileChannels - 1) / S::kTileChannels);
+    const int64_t clusters = kMode == kSplit ? tiles : std::min<int64_t>(o.sms / cluster, tiles);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = o.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    config.attrs = attr;
+    config.numAttrs = kMode == kOne ? 0 : 1;
+    return cudaLaunchKernelEx(&config, kernel, tw, tx, a, cluster);
+}
+
+// Which tile, and whether CTAs share one.  Tall tiles read each weight fewer times and feed the tensor
+// cores from fewer shared-memory bytes; a product that has too few of them for the SMs takes lower
+// tiles, and one that has few even then divides kdim.
 template <typename T>
-cudaError_t Launch(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const MatmulArgs& a, int sms, cudaStream_t s) {
+cudaError_t Launch(const Operands& o, const MatmulArgs& a) {
     if (a.kdim == 0) {
-        BiasRowsKernel<T><<<sms * 4, 256, 0, s>>>(a);
+        BiasRowsKernel<T><<<o.sms * 4, 256, 0, o.stream>>>(a);
         return cudaGetLastError();
     }
-    CUtensorMap tw;
-    if (!MakeMap(&tw, w, static_cast<int64_t>(a.experts) * a.n, a.kdim, ldw, kChannels)) return cudaErrorInvalidValue;
+    const int64_t ct = (a.n + kChannels - 1) / kChannels, nk = (a.kdim + kTileK - 1) / kTileK;
     const int64_t mean = (a.rows + a.experts - 1) / a.experts;
-    if (mean <= 16) return LaunchRows<16, T>(tw, q, ldq, a, sms, s);
-    if (mean <= 32) return LaunchRows<32, T>(tw, q, ldq, a, sms, s);
-    if (mean <= 64) return LaunchRows<64, T>(tw, q, ldq, a, sms, s);
-    if (mean <= 128) return LaunchRows<128, T>(tw, q, ldq, a, sms, s);
-    return LaunchRows<256, T>(tw, q, ldq, a, sms, s);
+    const auto fills = [&](int height) { return (a.rows + height - 1) / height * ct >= o.sms; };
+    if (mean > 128 && fills(256)) return LaunchTiles<256, kPair, T>(o, a, 2);
+    if (mean > 64 && fills(128)) return LaunchTiles<128, kOne, T>(o, a, 1);
+    if (mean > 32 && fills(64)) return LaunchTiles<64, kOne, T>(o, a, 1);
+    int height = mean > 64 ? 64 : mean > 16 ? 32 : 16;
+    const int64_t tiles = MostRowTiles(a, height) * ct;
+    // As many parts as there are SMs for them, of at least two steps of kdim.
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= o.sms && nk >= parts * 4) parts *= 2;
+    if (parts > 1) {
+        if (height == 128) return LaunchTiles<128, kSplit, T>(o, a, parts);
+        if (height == 16) return LaunchTiles<16, kSplit, T>(o, a, parts);
+        if (height == 32) return LaunchTiles<32, kSplit, T>(o, a, parts);
+        return LaunchTiles<64, kSplit, T>(o, a, parts);
+    }
+    if (height == 16) return LaunchTiles<16, kOne, T>(o, a, 1);
+    if (height == 32) return LaunchTiles<32, kOne, T>(o, a, 1);
+    return LaunchTiles<64, kOne, T>(o, a, 1);
 }
 
 int Bad(const char* msg) { return SetError(STLQ_B200_EINVAL, msg); }
@@ -375,12 +524,12 @@ int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_sc
         return Bad("a scale, bias, offsets or out pointer is not aligned to its element");
     DeviceScope scope(k->device);
     if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
     const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, out, ldo,
                        static_cast<unsigned int*>(k->err.p)};
-    if (out_dtype == STLQ_B200_F32) return Ck(Launch<float>(q, ldq, w, ldw, a, k->num_sms, s), "matmul_i8");
-    if (out_dtype == STLQ_B200_BF16) return Ck(Launch<__nv_bfloat16>(q, ldq, w, ldw, a, k->num_sms, s), "matmul_i8");
-    return Ck(Launch<__half>(q, ldq, w, ldw, a, k->num_sms, s), "matmul_i8");
+    const Operands o{q, ldq, w, ldw, k->num_sms, static_cast<cudaStream_t>(stream)};
+    if (out_dtype == STLQ_B200_F32) return Ck(Launch<float>(o, a), "matmul_i8");
+    if (out_dtype == STLQ_B200_BF16) return Ck(Launch<__nv_bfloat16>(o, a), "matmul_i8");
+    return Ck(Launch<__half>(o, a), "matmul_i8");
 }
 
 template <typename F>
