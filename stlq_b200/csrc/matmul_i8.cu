@@ -204,67 +204,96 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Rows of a tile's MMA: what is left of the segment, rounded up.
     auto columns = [](const Tile& t) { return min(kRows, (t.end - t.row0 + S::kGranule - 1) / S::kGranule * S::kGranule); };
 
-    if (warp == 0 && lane == 0) {
-        int step = 0;
+    // The two warps that load and multiply run converged, with one lane issuing: addresses and
+    // descriptors then stay in uniform registers, and a step costs the issuing thread few instructions
+    // (with a loop of lane 0's own, a step of four MMAs took 285 ns whatever the tile).
+    if (warp == 0) {
+        const bool one = tc::ElectOne();
+        int s = 0, used = 0;         // the stage, and how many have been filled
+        uint32_t parity = 1;         // of the wait for its last use
         bool ok = true;
         for (int id = first_tile; id < tiles && ok; id += tile_step) {
             const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
             const int wrow = t.expert * a.n + t.channel0 + (kMode == kPair ? rank * kChannels : 0);
             const int xrow = t.row0 + (kMode == kPair ? rank * (columns(t) / 2) : 0);
-            for (int kb = k_first; kb < k_last; ++kb, ++step) {
-                const int s = step % S::kStages, round = step / S::kStages;
-                if (round > 0 && !(ok = tc::MbarWait(&empty[s], (round - 1) & 1, a.err, kWaitNs))) break;
+            for (int kb = k_first; kb < k_last; ++kb) {
+                if (used >= S::kStages && !(ok = __all_sync(0xffffffffu, tc::MbarWait(&empty[s], parity, a.err, kWaitNs)))) break;
                 unsigned char* st = base + s * S::kStageBytes;
-                if constexpr (kMode == kPair) {
-                    // The even CTA's barrier counts the bytes of both.
-                    if (rank == 0) tc::MbarArriveExpectTx(&full[s], 2 * S::kStageBytes);
-                    const uint32_t bar = tc::ClusterAddr(&full[s], 0);
-                    tc::TmaLoad2dPair(st, &tw, bar, kb * kTileK, wrow);
-                    tc::TmaLoad2dPair(st + kWBytes, &tx, bar, kb * kTileK, xrow);
-                } else {
-                    tc::MbarArriveExpectTx(&full[s], S::kStageBytes);
-                    tc::TmaLoad2d(st, &tw, &full[s], kb * kTileK, wrow);
-                    tc::TmaLoad2d(st + kWBytes, &tx, &full[s], kb * kTileK, xrow);
+                if (one) {
+                    if constexpr (kMode == kPair) {
+                        // The even CTA's barrier counts the bytes of both.
+                        if (rank == 0) tc::MbarArriveExpectTx(&full[s], 2 * S::kStageBytes);
+                        const uint32_t bar = tc::ClusterAddr(&full[s], 0);
+                        tc::TmaLoad2dPair(st, &tw, bar, kb * kTileK, wrow);
+                        tc::TmaLoad2dPair(st + kWBytes, &tx, bar, kb * kTileK, xrow);
+                    } else {
+                        tc::MbarArriveExpectTx(&full[s], S::kStageBytes);
+                        tc::TmaLoad2d(st, &tw, &full[s], kb * kTileK, wrow);
+                        tc::TmaLoad2d(st + kWBytes, &tx, &full[s], kb * kTileK, xrow);
+                    }
+                }
+                __syncwarp();
+                used = min(used + 1, 2 * S::kStages);
+                if (++s == S::kStages) {
+                    s = 0;
+                    parity ^= 1;
                 }
             }
         }
-        // Copies still in flight land before the block may exit.
+        // Copies still in flight land before the block may exit: the last use of each stage.
         if (kMode != kPair || rank == 0)
-            for (int i = step - 1; i >= 0 && i >= step - S::kStages; --i)
-                tc::MbarWait(&full[i % S::kStages], (i / S::kStages) & 1, a.err, kWaitNs, false);
+            for (int i = 0; i < min(used, S::kStages); ++i) {
+                if (--s < 0) {
+                    s = S::kStages - 1;
+                    parity ^= 1;
+                }
+                tc::MbarWait(&full[s], parity ^ 1, a.err, kWaitNs, false);
+            }
         if (kMode == kPair && !ok) {  // the other CTA's barrier says no more: leave them 10 ms
             const uint64_t t0 = tc::GlobalTimerNs();
             while (tc::GlobalTimerNs() - t0 < 10000000ull) {
             }
         }
-    } else if (warp == 1 && lane == 0 && (kMode != kPair || rank == 0)) {
-        int step = 0, done = 0;
+    } else if (warp == 1 && (kMode != kPair || rank == 0)) {
+        const bool one = tc::ElectOne();
+        const uint64_t dw0 = tc::SmemDescSw128(tc::SmemAddr(base)), dx0 = tc::SmemDescSw128(tc::SmemAddr(base) + kWBytes);
+        int s = 0, done = 0;
+        uint32_t parity = 0;
         bool ok = true;
         for (int id = first_tile; id < tiles && ok; id += tile_step, ++done) {
             const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
             const uint32_t idesc = tc::InstrDescI8(S::kTileChannels, columns(t));
             const int b = kMode == kSplit ? 0 : done & 1, use = done >> 1;
-            if (use > 0 && !(ok = tc::MbarWait(&taken[b], (use - 1) & 1, a.err, kWaitNs))) break;
+            if (use > 0 && !(ok = __all_sync(0xffffffffu, tc::MbarWait(&taken[b], (use - 1) & 1, a.err, kWaitNs)))) break;
             tc::FenceAfterSync();
-            for (int kb = k_first; kb < k_last; ++kb, ++step) {
-                const int s = step % S::kStages;
-                if (!(ok = tc::MbarWait(&full[s], (step / S::kStages) & 1, a.err, kWaitNs))) break;
+            const uint32_t to = tmem + b * S::kColumns;
+            uint32_t more = 0;
+            for (int kb = k_first; kb < k_last; ++kb) {
+                if (!(ok = __all_sync(0xffffffffu, tc::MbarWait(&full[s], parity, a.err, kWaitNs)))) break;
                 tc::FenceAfterSync();
-                const uint32_t w = tc::SmemAddr(base + s * S::kStageBytes), x = w + kWBytes;
+                // Addresses in a descriptor count 16-byte units: a step of 32 bytes of kdim is 2.
+                const uint64_t dw = dw0 + s * (S::kStageBytes >> 4), dx = dx0 + s * (S::kStageBytes >> 4);
+                if (one) {
 #pragma unroll
-                for (int k = 0; k < kTileK / 32; ++k) {
-                    const uint64_t dw = tc::SmemDescSw128(w + k * 32), dx = tc::SmemDescSw128(x + k * 32);
-                    const uint32_t more = (kb > k_first || k > 0) ? 1u : 0u;
-                    if constexpr (kMode == kPair) tc::UmmaI8Pair(tmem + b * S::kColumns, dw, dx, idesc, more);
-                    else tc::UmmaI8(tmem + b * S::kColumns, dw, dx, idesc, more);
+                    for (int k = 0; k < kTileK / 32; ++k) {
+                        if constexpr (kMode == kPair) tc::UmmaI8Pair(to, dw + 2 * k, dx + 2 * k, idesc, k ? 1u : more);
+                        else tc::UmmaI8(to, dw + 2 * k, dx + 2 * k, idesc, k ? 1u : more);
+                    }
+                    if constexpr (kMode == kPair) tc::UmmaCommitPair(&empty[s]);
+                    else tc::UmmaCommit(&empty[s]);
                 }
-                if constexpr (kMode == kPair) tc::UmmaCommitPair(&empty[s]);
-                else tc::UmmaCommit(&empty[s]);
+                __syncwarp();
+                more = 1;
+                if (++s == S::kStages) {
+                    s = 0;
+                    parity ^= 1;
+                }
             }
-            if (ok) {
+            if (ok && one) {
                 if constexpr (kMode == kPair) tc::UmmaCommitPair(&made[b]);
                 else tc::UmmaCommit(&made[b]);
             }
+            __syncwarp();
         }
     } else if (warp >= 2) {
         const int quarter = warp & 3;  // the TMEM lanes this warp may read

@@ -39,6 +39,17 @@ __device__ __forceinline__ bool MbarTryWait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
+// One lane of a converged warp, the same one each time.
+__device__ __forceinline__ bool ElectOne() {
+    uint32_t ok = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok));
+    return ok != 0;
+}
+
 __device__ __forceinline__ uint64_t GlobalTimerNs() {
     uint64_t t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -51,16 +62,21 @@ __device__ __forceinline__ uint64_t GlobalTimerNs() {
 // copies in flight pass false, so that the CTA never exits while a copy still writes its memory.
 __device__ __forceinline__ bool MbarWait(uint64_t* bar, uint32_t parity, unsigned int* err, uint64_t limit_ns,
                                          bool abort_on_err = true) {
-    if (MbarTryWait(bar, parity)) return true;
+    // The flag is a trip to L2 and the timer is slow to read: they are looked at once in many tries, as
+    // a try itself lasts from a few to some thousand cycles.
+    constexpr int kTries = 256;
+    for (int i = 0; i < kTries; ++i)
+        if (MbarTryWait(bar, parity)) return true;
     const uint64_t t0 = GlobalTimerNs();
-    while (!MbarTryWait(bar, parity)) {
+    for (;;) {
+        for (int i = 0; i < kTries; ++i)
+            if (MbarTryWait(bar, parity)) return true;
         if ((abort_on_err && (*reinterpret_cast<volatile unsigned int*>(err) & kErrWaitTimeout)) ||
             GlobalTimerNs() - t0 > limit_ns) {
             atomicOr(err, static_cast<unsigned int>(kErrWaitTimeout));
             return false;
         }
     }
-    return true;
 }
 
 // 2-D TMA tile load into shared memory, completing on `bar` (byte count set by expect_tx).
