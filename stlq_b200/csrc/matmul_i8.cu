@@ -29,10 +29,10 @@ namespace tc = stlq_b200::tc;
 constexpr int kChannels = 128;                       // channels of a CTA's tile (its share of the MMA's M)
 constexpr int kTileK = 128;                          // bytes of a 128-byte swizzle row
 constexpr uint32_t kWBytes = kChannels * kTileK;
-constexpr int kWriters = 8;                          // warps of the epilogue, two for each quarter of the TMEM lanes
+constexpr int kWriters = 8;                          // warps of the epilogue
+constexpr int kShare = kWriters / 4;                 // of them, those of a quarter of the TMEM lanes
 constexpr int kThreads = 64 + 32 * kWriters;         // warp 0 loads, warp 1 multiplies, the others write
 constexpr uint64_t kWaitNs = 2000000000ull;          // 2 s per barrier wait
-constexpr int kBand = 8;                             // row tiles that run side by side over the channels
 
 // kOne: a CTA computes tiles of its own, one after the other.  kPair: two CTAs share a tile of 256
 // channels (tcgen05 cta_group::2): each holds its channels and half of the rows, so that an operand
@@ -40,14 +40,18 @@ constexpr int kBand = 8;                             // row tiles that run side 
 // for one tile and add up over distributed shared memory, for products with few tiles.
 enum Mode { kOne, kPair, kSplit };
 
-template <int kRows, Mode kMode>
+template <int kRows, Mode kMode, typename T>
 struct Shape {
     static constexpr uint32_t kXBytes = (kMode == kPair ? kRows / 2 : kRows) * kTileK;
     static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
-    static constexpr int kStages = std::min<int>(10, 200 * 1024 / kStageBytes);
+    // Where a writing warp lays out 16 rows of its 32 channels for a TMA store, twice.
+    static constexpr uint32_t kOutBytes = 16 * 32 * sizeof(T);
+    static constexpr uint32_t kAllOut = kMode == kSplit ? 0 : 2 * kWriters * kOutBytes;
+    static constexpr int kStages = std::min<int>(10, (209 * 1024 - kAllOut) / kStageBytes);
     static constexpr int kColumns = kRows < 32 ? 32 : kRows;        // TMEM columns of one accumulator
     static constexpr uint32_t kTmem = (kMode == kSplit ? 1 : 2) * kColumns;  // two: one is written out while the next is made
     static constexpr int kTileChannels = kMode == kPair ? 2 * kChannels : kChannels;
+    static constexpr int kOwnRows = std::max(16, kRows / kShare);   // rows of the tile that a writing warp takes
     static constexpr int kGranule = kMode == kPair ? 32 : 16;       // rows of an MMA come in multiples of this
 };
 
@@ -57,6 +61,8 @@ struct MatmulArgs {
     const float* bias;
     const int* offsets;  // null: one matrix, all rows
     int experts, rows, n, kdim;
+    int tma_out;         // the output's rows begin on 16-byte boundaries
+    int band;            // row tiles that run side by side over the channels
     void* out;
     int64_t ldo;
     unsigned int* err;
@@ -104,31 +110,32 @@ __device__ __forceinline__ Tile FindTile(const MatmulArgs& a, const Segments& sg
         t.row0 = 0;
         t.end = a.rows;
     }
-    // Bands of kBand row tiles, the band's row tiles running fastest: the tiles in flight share few
-    // rows and few channels, which stay in L2.
+    // Bands of row tiles, the band's row tiles running fastest: the tiles in flight share few rows and
+    // few channels, which stay in L2.
     const int rt = (t.end - t.row0 + kRows - 1) / kRows;
-    const int band = local / (kBand * ct), in = local - band * kBand * ct;
-    const int height = min(kBand, rt - band * kBand);
+    const int band = local / (a.band * ct), in = local - band * a.band * ct;
+    const int height = min(a.band, rt - band * a.band);
     t.channel0 = in / height * kTileChannels;
-    t.row0 += (band * kBand + in % height) * kRows;
+    t.row0 += (band * a.band + in % height) * kRows;
     return t;
 }
 
 template <int kRows, Mode kMode, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
-    MatmulI8Kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const MatmulArgs a,
-                   int cluster) {
-    using S = Shape<kRows, kMode>;
+    MatmulI8Kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+                   const __grid_constant__ CUtensorMap to, const MatmulArgs a, int cluster) {
+    using S = Shape<kRows, kMode, T>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = smem_raw + ((1024 - (tc::SmemAddr(smem_raw) & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(base + S::kStages * S::kStageBytes);
+    unsigned char* outs = base + S::kStages * S::kStageBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(outs + S::kAllOut);
     uint64_t* empty = full + S::kStages;
     uint64_t* made = empty + S::kStages;  // an accumulator is complete
     uint64_t* taken = made + 2;           // an accumulator has been read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
-    float* row_scales = reinterpret_cast<float*>(tmem_slot + 4);  // [kWriters][kRows]
+    float* row_scales = reinterpret_cast<float*>(tmem_slot + 4);  // [kWriters][kOwnRows]
     Segments sg;
-    sg.first = reinterpret_cast<int*>(row_scales + kWriters * kRows);
+    sg.first = reinterpret_cast<int*>(row_scales + kWriters * S::kOwnRows);
     sg.begin = sg.first + (a.experts + 1);
     sg.end = sg.begin + a.experts;
 
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int b = kMode == kSplit ? 0 : done & 1, use = done >> 1;
             if (use > 0 && !(ok = __all_sync(0xffffffffu, tc::MbarWait(&taken[b], (use - 1) & 1, a.err, kWaitNs)))) break;
             tc::FenceAfterSync();
-            const uint32_t to = tmem + b * S::kColumns;
+            const uint32_t acc = tmem + b * S::kColumns;
             uint32_t more = 0;
             for (int kb = k_first; kb < k_last; ++kb) {
                 if (!(ok = __all_sync(0xffffffffu, tc::MbarWait(&full[s], parity, a.err, kWaitNs)))) break;
@@ -276,8 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (one) {
 #pragma unroll
                     for (int k = 0; k < kTileK / 32; ++k) {
-                        if constexpr (kMode == kPair) tc::UmmaI8Pair(to, dw + 2 * k, dx + 2 * k, idesc, k ? 1u : more);
-                        else tc::UmmaI8(to, dw + 2 * k, dx + 2 * k, idesc, k ? 1u : more);
+                        if constexpr (kMode == kPair) tc::UmmaI8Pair(acc, dw + 2 * k, dx + 2 * k, idesc, k ? 1u : more);
+                        else tc::UmmaI8(acc, dw + 2 * k, dx + 2 * k, idesc, k ? 1u : more);
                     }
                     if constexpr (kMode == kPair) tc::UmmaCommitPair(&empty[s]);
                     else tc::UmmaCommit(&empty[s]);
@@ -298,24 +305,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp >= 2) {
         const int quarter = warp & 3;  // the TMEM lanes this warp may read
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const int half = (warp - 2) >> 2;  // its 16 columns of every 32
-        float* scales = row_scales + (warp - 2) * kRows;
+        // Of every 16 * kShare rows, this warp takes 16.
+        constexpr int kStep = 16 * kShare;
+        const int share = (warp - 2) >> 2;
+        float* scales = row_scales + (warp - 2) * S::kOwnRows;
         int* parts = reinterpret_cast<int*>(base);  // kSplit: [kRows][kChannels] over the stages, once they are read
         T* out = static_cast<T*>(a.out);
-        int done = 0;
+        int done = 0, slot = 0;
         bool ok = true;
+        const bool one = tc::ElectOne();
+        // What a tile needs beside its sums.  The next tile's is on its way while this one is written:
+        // with few steps of kdim a tile would otherwise wait for it every time.
+        constexpr int kOwn = (S::kOwnRows + 31) / 32;
+        struct Side {
+            Tile t;
+            float ws, bias, qs[kOwn];
+        };
+        auto fetch = [&](int id) {
+            Side x;
+            x.t = FindTile<kRows, S::kTileChannels>(a, sg, id);
+            const int c = x.t.channel0 + (kMode == kPair ? rank * kChannels : 0) + quarter * 32 + lane;
+            const int64_t wc = static_cast<int64_t>(x.t.expert) * a.n + c;
+            x.ws = c < a.n ? a.w_scale[wc] : 0.0f;
+            x.bias = c < a.n && a.bias ? a.bias[wc] : 0.0f;
+            const int count = min(kRows, x.t.end - x.t.row0);
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                const int r = i * 32 + lane, row = (r >> 4) * kStep + share * 16 + (r & 15);
+                x.qs[i] = r < S::kOwnRows && row < count ? a.q_scale[x.t.row0 + row] : 0.0f;
+            }
+            return x;
+        };
+        Side next{};
+        if (first_tile < tiles) next = fetch(first_tile);
         for (int id = first_tile; id < tiles && ok; id += tile_step, ++done) {
-            const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
+            const Side now = next;
+            const Tile t = now.t;
+            const float ws = now.ws, bias = now.bias;
+            if (kMode != kSplit && id + tile_step < tiles) next = fetch(id + tile_step);
             const int b = kMode == kSplit ? 0 : done & 1;
             const int c = t.channel0 + (kMode == kPair ? rank * kChannels : 0) + quarter * 32 + lane;
             const bool real = c < a.n;
-            const int64_t wc = static_cast<int64_t>(t.expert) * a.n + c;
-            const float ws = real ? a.w_scale[wc] : 0.0f;
-            const float bias = real && a.bias ? a.bias[wc] : 0.0f;
             const int count = min(kRows, t.end - t.row0);
-            for (int r = lane; r < count; r += 32) scales[r] = a.q_scale[t.row0 + r];
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i)
+                if (i * 32 + lane < S::kOwnRows) scales[i * 32 + lane] = now.qs[i];
             __syncwarp();
-            T* to = out + (static_cast<int64_t>(t.row0) + half * 16) * a.ldo + c;
+            T* direct = out + (static_cast<int64_t>(t.row0) + share * 16) * a.ldo + c;
             ok = __all_sync(0xffffffffu, tc::MbarWait(&made[b], (done >> 1) & 1, a.err, kWaitNs));
             if (ok) {
                 tc::FenceAfterSync();
@@ -326,34 +362,58 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int j = 0; j < 16; ++j) parts[(c0 + j) * kChannels + quarter * 32 + lane] = v[j];
                     } else {
                         float y[16];
+                        const float4* own = reinterpret_cast<const float4*>(scales + c0 / kShare / 16 * 16);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) y[j] = fmaf(__int2float_rn(v[j]) * scales[c0 + j], ws, bias);
-                        const int left = real ? count - c0 : 0;
-                        T* row = to;
-                        if (left >= 16) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j, row += a.ldo) *row = Out<T>(y[j]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j, row += a.ldo)
-                                if (j < left) *row = Out<T>(y[j]);
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 sc = own[j / 4];
+                            y[j] = fmaf(__int2float_rn(v[j]) * sc.x, ws, bias);
+                            y[j + 1] = fmaf(__int2float_rn(v[j + 1]) * sc.y, ws, bias);
+                            y[j + 2] = fmaf(__int2float_rn(v[j + 2]) * sc.z, ws, bias);
+                            y[j + 3] = fmaf(__int2float_rn(v[j + 3]) * sc.w, ws, bias);
                         }
-                        to += 32 * a.ldo;
+                        // 16 rows of this segment at once by TMA, which also leaves out what is past the
+                        // output's edges; rows that belong to the next segment are left out here.
+                        if (a.tma_out && (c0 + 16 <= count || !a.offsets)) {
+                            T* lay = reinterpret_cast<T*>(outs + (2 * (warp - 2) + slot) * S::kOutBytes);
+                            if (one) tc::BulkWaitRead<1>();
+                            __syncwarp();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) lay[j * 32 + lane] = Out<T>(y[j]);
+                            tc::FenceAsyncShared();
+                            __syncwarp();
+                            if (one) {
+                                tc::TmaStore2d(&to, lay, c - lane, t.row0 + c0);
+                                tc::BulkCommit();
+                            }
+                            slot ^= 1;
+                        } else {
+                            const int left = real ? count - c0 : 0;
+                            T* row = direct;
+                            if (left >= 16) {
+#pragma unroll
+                                for (int j = 0; j < 16; ++j, row += a.ldo) *row = Out<T>(y[j]);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 16; ++j, row += a.ldo)
+                                    if (j < left) *row = Out<T>(y[j]);
+                            }
+                        }
+                        direct += kStep * a.ldo;
                     }
                 };
                 // The next 16 columns are on their way while 16 are written.
                 int va[16], vb[16];
-                int c0 = half * 16;
+                int c0 = share * 16;
                 if (c0 < count) tc::TmemLoad16(from + c0, va);
 #pragma unroll 1
-                for (; c0 < count; c0 += 64) {
+                for (; c0 < count; c0 += 2 * kStep) {
                     tc::TmemLoadWait(va);
-                    if (c0 + 32 < count) tc::TmemLoad16(from + c0 + 32, vb);
+                    if (c0 + kStep < count) tc::TmemLoad16(from + c0 + kStep, vb);
                     write(va, c0);
-                    if (c0 + 32 >= count) break;
+                    if (c0 + kStep >= count) break;
                     tc::TmemLoadWait(vb);
-                    if (c0 + 64 < count) tc::TmemLoad16(from + c0 + 64, va);
-                    write(vb, c0 + 32);
+                    if (c0 + 2 * kStep < count) tc::TmemLoad16(from + c0 + 2 * kStep, va);
+                    write(vb, c0 + kStep);
                 }
                 tc::FenceBeforeSync();
             }
@@ -364,9 +424,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else tc::MbarArrive(&taken[b]);
             }
         }
+        if (kMode != kSplit && one) tc::BulkWaitAll();  // before the memory that they read goes
     }
     if constexpr (kMode == kSplit) {
-        // Row j of the tile is finished by CTA j % cluster: the parts in order of kdim.  A quarter's two
+        // Row j of the tile is finished by CTA j % cluster: the parts in order of kdim.  A quarter's
         // warps take these rows in turn.
         tc::FenceBeforeSync();
         __syncwarp();
@@ -378,13 +439,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int count = min(kRows, t.end - t.row0);
             if (c < a.n) {
                 const float ws = a.w_scale[wc], bias = a.bias ? a.bias[wc] : 0.0f;
-                const float* scales = row_scales + (warp - 2) * kRows;
-                for (int j = rank + cluster * ((warp - 2) >> 2); j < count; j += 2 * cluster) {
+                for (int j = rank + cluster * ((warp - 2) >> 2); j < count; j += kShare * cluster) {
+                    const float scale = a.q_scale[t.row0 + j];
                     int sum = 0;
 #pragma unroll 8
                     for (int r = 0; r < cluster; ++r) sum += tc::LoadCluster(tc::ClusterAddr(base, r) + (j * kChannels + at) * 4);
                     static_cast<T*>(a.out)[(static_cast<int64_t>(t.row0) + j) * a.ldo + c] =
-                        Out<T>(fmaf(__int2float_rn(sum) * scales[j], ws, bias));
+                        Out<T>(fmaf(__int2float_rn(sum) * scale, ws, bias));
                 }
             }
         }
@@ -444,17 +505,19 @@ PFN_cuTensorMapEncodeTiled_v12000 EncodeFn() {
     return fn;
 }
 
-// Row-major rows x kdim bytes, boxes of box_rows x 128 bytes, 128-byte swizzle, zeros out of bounds.
-bool MakeMap(CUtensorMap* map, const int8_t* p, int64_t rows, int kdim, int64_t ld, int box_rows) {
+// Row-major rows x cols elements, row_bytes apart, in boxes of box_rows x box_cols; zeros out of bounds.
+// The 8-bit operands come with the 128-byte swizzle, the output without one.
+bool MakeMap(CUtensorMap* map, CUtensorMapDataType type, const void* p, int64_t rows, int cols, int64_t row_bytes, int box_rows,
+             int box_cols) {
     const auto fn = EncodeFn();
     if (!fn) return false;
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(kdim), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
-    const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)};
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t estride[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dims, strides, box, estride,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return fn(map, type, 2, const_cast<void*>(p), dims, strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              type == CU_TENSOR_MAP_DATA_TYPE_UINT8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct Operands {
@@ -472,15 +535,28 @@ int64_t MostRowTiles(const MatmulArgs& a, int height) {
     return a.offsets ? std::min<int64_t>(a.rows, full + a.experts) : full;
 }
 
+// And how many are likely: every expert that can have a row ends in a part of a tile.
+int64_t LikelyRowTiles(const MatmulArgs& a, int height) {
+    if (!a.offsets) return MostRowTiles(a, height);
+    const int64_t used = std::min(a.rows, a.experts);
+    return std::max<int64_t>(used, a.rows / height + used / 2);
+}
+
 template <int kRows, Mode kMode, typename T>
 cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
-    using S = Shape<kRows, kMode>;
-    CUtensorMap tw, tx;
-    if (!MakeMap(&tw, o.w, static_cast<int64_t>(a.experts) * a.n, a.kdim, o.ldw, kChannels) ||
-        !MakeMap(&tx, o.q, a.rows, a.kdim, o.ldq, kMode == kPair ? kRows / 2 : kRows))
+    using S = Shape<kRows, kMode, T>;
+    CUtensorMap tw, tx, to{};
+    if (!MakeMap(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.w, static_cast<int64_t>(a.experts) * a.n, a.kdim, o.ldw, kChannels, kTileK) ||
+        !MakeMap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.q, a.rows, a.kdim, o.ldq, kMode == kPair ? kRows / 2 : kRows, kTileK))
         return cudaErrorInvalidValue;
-    const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + (2 * S::kStages + 4) * 8 + 16 + 4 * kWriters * kRows +
-                        (a.offsets ? (3 * static_cast<size_t>(a.experts) + 1) * 4 : 0);
+    constexpr auto kOutType = sizeof(T) == 4                       ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                              : std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (kMode != kSplit && a.tma_out &&
+        !MakeMap(&to, kOutType, a.out, a.rows, a.n, a.ldo * static_cast<int64_t>(sizeof(T)), 16, 32))
+        return cudaErrorInvalidValue;
+    const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kAllOut + (2 * S::kStages + 4) * 8 + 16 +
+                        4 * kWriters * S::kOwnRows + (a.offsets ? (3 * static_cast<size_t>(a.experts) + 1) * 4 : 0);
     const auto kernel = MatmulI8Kernel<kRows, kMode, T>;
     if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); e != cudaSuccess) return e;
     const int64_t tiles = MostRowTiles(a, kRows) * ((a.n + S::kTileChannels - 1) / S::kTileChannels);
@@ -495,38 +571,65 @@ cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
     attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
     config.attrs = attr;
     config.numAttrs = kMode == kOne ? 0 : 1;
-    return cudaLaunchKernelEx(&config, kernel, tw, tx, a, cluster);
+    return cudaLaunchKernelEx(&config, kernel, tw, tx, to, a, cluster);
 }
 
-// Which tile, and whether CTAs share one.  Tall tiles read each weight fewer times and feed the tensor
-// cores from fewer shared-memory bytes; a product that has too few of them for the SMs takes lower
-// tiles, and one that has few even then divides kdim.
+template <typename T>
+cudaError_t LaunchAs(const Operands& o, const MatmulArgs& a, Mode mode, int height, int parts) {
+    if (mode == kPair) return LaunchTiles<256, kPair, T>(o, a, 2);
+    if (mode == kOne) {
+        if (height == 16) return LaunchTiles<16, kOne, T>(o, a, 1);
+        if (height == 32) return LaunchTiles<32, kOne, T>(o, a, 1);
+        if (height == 64) return LaunchTiles<64, kOne, T>(o, a, 1);
+        return LaunchTiles<128, kOne, T>(o, a, 1);
+    }
+    if (height == 16) return LaunchTiles<16, kSplit, T>(o, a, parts);
+    if (height == 32) return LaunchTiles<32, kSplit, T>(o, a, parts);
+    return LaunchTiles<64, kSplit, T>(o, a, parts);
+}
+
+// Which tile, and whether CTAs share one: the least of the times that a call is expected to take, in
+// microseconds, fitted to what was measured on B200.  A wave of tiles h rows high takes
+// 0.22 us + 0.4 ns h for every 128 terms (issuing the loads and MMAs bounds it, hence so little of the
+// height) and 0.5 us + 8.6 ns h beside them; a wave of pairs 0.235 and 3.6 us.  A kernel without work takes
+// 2.4 us, one of pairs 5; adding up the parts of a tile 3 us, 50 ns a row and 10 ns a row of its height.
+// Measured at both sides of the borders (rows x n x kdim): 128 x 4,096 x 4,096, one 64 high 10.9 us, two
+// parts 12.7; 16 x 4,096 x 4,096, four parts 7.7, one 10.0; 1,024 x 4,096 x 4,096, pairs 16.8, one 128 high
+// 21; 8,000 x 8,000 x 1,000, pairs 83, one 128 high 104; 4,096 x 1,024 x 1,024, both 9.3;
+// 4,096 x 65,536 x 128 to 32 bits, one 128 high 200, pairs 236.
 template <typename T>
 cudaError_t Launch(const Operands& o, const MatmulArgs& a) {
     if (a.kdim == 0) {
         BiasRowsKernel<T><<<o.sms * 4, 256, 0, o.stream>>>(a);
         return cudaGetLastError();
     }
-    const int64_t ct = (a.n + kChannels - 1) / kChannels, nk = (a.kdim + kTileK - 1) / kTileK;
-    const int64_t mean = (a.rows + a.experts - 1) / a.experts;
-    const auto fills = [&](int height) { return (a.rows + height - 1) / height * ct >= o.sms; };
-    if (mean > 128 && fills(256)) return LaunchTiles<256, kPair, T>(o, a, 2);
-    if (mean > 64 && fills(128)) return LaunchTiles<128, kOne, T>(o, a, 1);
-    if (mean > 32 && fills(64)) return LaunchTiles<64, kOne, T>(o, a, 1);
-    int height = mean > 64 ? 64 : mean > 16 ? 32 : 16;
-    const int64_t tiles = MostRowTiles(a, height) * ct;
-    // As many parts as there are SMs for them, of at least two steps of kdim.
-    int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= o.sms && nk >= parts * 4) parts *= 2;
-    if (parts > 1) {
-        if (height == 128) return LaunchTiles<128, kSplit, T>(o, a, parts);
-        if (height == 16) return LaunchTiles<16, kSplit, T>(o, a, parts);
-        if (height == 32) return LaunchTiles<32, kSplit, T>(o, a, parts);
-        return LaunchTiles<64, kSplit, T>(o, a, parts);
+    const int64_t ct = (a.n + kChannels - 1) / kChannels;
+    const int nk = (a.kdim + kTileK - 1) / kTileK;
+    Mode mode = kOne;
+    int best_height = 128, best_parts = 1;
+    double best = 1e300;
+    const auto take = [&](double us, Mode m, int height, int parts) {
+        if (us < best) {
+            best = us;
+            mode = m;
+            best_height = height;
+            best_parts = parts;
+        }
+    };
+    const auto waves = [](int64_t tiles, int64_t at_once) { return static_cast<double>((tiles + at_once - 1) / at_once); };
+    for (int height = 128; height >= 16; height /= 2) {
+        const double step = 0.22 + 0.0004 * height, write = 0.5 + 0.0086 * height;
+        take(2.4 + waves(LikelyRowTiles(a, height) * ct, o.sms) * (step * nk + write), kOne, height, 1);
+        if (height > 64) continue;
+        const int64_t most = MostRowTiles(a, height) * ct;
+        for (int parts = 2; parts <= 8 && nk >= 2 * parts; parts *= 2) {
+            // Clusters of eight find room on fewer SMs: 16 of them did not run at once, 12 did.
+            if (most * parts > (parts == 8 ? o.sms * 2 / 3 : o.sms * 7 / 8)) break;
+            take(2.4 + step * ((nk + parts - 1) / parts) + 3.0 + 0.05 * std::min(a.rows, height) + 0.01 * height, kSplit, height, parts);
+        }
     }
-    if (height == 16) return LaunchTiles<16, kOne, T>(o, a, 1);
-    if (height == 32) return LaunchTiles<32, kOne, T>(o, a, 1);
-    return LaunchTiles<64, kOne, T>(o, a, 1);
+    take(5.0 + waves(LikelyRowTiles(a, 256) * ((a.n + 255) / 256), o.sms / 2) * (0.235 * nk + 3.6), kPair, 256, 2);
+    return LaunchAs<T>(o, a, mode, best_height, best_parts);
 }
 
 int Bad(const char* msg) { return SetError(STLQ_B200_EINVAL, msg); }
@@ -546,6 +649,7 @@ int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_sc
     if (rows > 0x7fffff00 || static_cast<int64_t>(experts) * n > 0x7fffff00) return Bad("rows and experts * n must be below 2^31 - 256");
     if (((rows + 15) / 16 + experts) * ((static_cast<int64_t>(n) + kChannels - 1) / kChannels) > 0x7fffff00)
         return Bad("rows * n too large for one call");
+    if (ldq >= (int64_t{1} << 40) || ldw >= (int64_t{1} << 40)) return Bad("ldq and ldw must be below 2^40");
     if (kdim > 0 && (!Aligned(q, 16) || !Aligned(w, 16) || ldq % 16 || ldw % 16))
         return Bad("q and w must be 16-byte aligned with ldq and ldw multiples of 16");
     if (!Aligned(q_scale, 4) || !Aligned(w_scale, 4) || !Aligned(bias, 4) || !Aligned(offsets, 4) ||
@@ -553,7 +657,10 @@ int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_sc
         return Bad("a scale, bias, offsets or out pointer is not aligned to its element");
     DeviceScope scope(k->device);
     if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
-    const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, out, ldo,
+    const int64_t out_bytes = out_dtype == STLQ_B200_F32 ? 4 : 2;
+    // TMA's rows: on 16-byte boundaries, less than 2^40 bytes apart.
+    const int tma_out = Aligned(out, 16) && ldo * out_bytes % 16 == 0 && ldo < (int64_t{1} << 37);
+    const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, tma_out, 8, out, ldo,
                        static_cast<unsigned int*>(k->err.p)};
     const Operands o{q, ldq, w, ldw, k->num_sms, static_cast<cudaStream_t>(stream)};
     if (out_dtype == STLQ_B200_F32) return Ck(Launch<float>(o, a), "matmul_i8");

@@ -88,6 +88,23 @@ __device__ __forceinline__ void TmaLoad2d(void* dst, const void* tmap, uint64_t*
         : "memory");
 }
 
+// 2-D TMA tile store out of shared memory.  The threads that wrote it fence (FenceAsyncShared) before
+// one of them stores; that one commits and waits for its groups.
+__device__ __forceinline__ void FenceAsyncShared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void TmaStore2d(const void* tmap, const void* src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(SmemAddr(src)), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void BulkCommit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// All but the last kLeft groups of this thread have read their shared memory.
+template <int kLeft>
+__device__ __forceinline__ void BulkWaitRead() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void BulkWaitAll() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // Shared-memory matrix descriptor for a K-major operand tile stored with the 128-byte swizzle:
 // rows of 128 bytes, 8-row core groups 1024 bytes apart (stride byte offset), descriptor version 1.
 __device__ __forceinline__ uint64_t SmemDescSw128(uint32_t saddr) {
