@@ -2,6 +2,8 @@
 
     python -m stlq_b200.build            # incremental
     python -m stlq_b200.build --force    # rebuild everything
+
+It also builds _operators.so, the Python binding of the routed 8-bit operators, against the installed torch.
 """
 from __future__ import annotations
 
@@ -9,10 +11,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libstlq_b200.so")
+BINDING = os.path.join(HERE, "binding", "operators.cpp")
+BINDING_OUT = os.path.join(HERE, "_operators.so")
 OBJDIR = os.path.join(HERE, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC = os.environ.get("NVCC", shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc")
@@ -55,5 +60,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return OUT
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    header = os.path.join(HERE, "..", "include", "stlq_b200.h")
+    if force or _stale(BINDING_OUT, [BINDING, header]):
+        import importlib.util
+
+        torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+        inc, lib = os.path.join(torch_dir, "include"), os.path.join(torch_dir, "lib")
+        cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(NVCC))), "include")
+        cmd = [HOST_CXX, "-O2", "-std=c++17", "-shared", "-fPIC", BINDING, "-o", BINDING_OUT, "-I", inc, "-I",
+               os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_path("include"), "-I", cuda, "-L", lib,
+               "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath," + lib]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+    return BINDING_OUT
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose=True)
+    build_binding(force="--force" in sys.argv, verbose=True)

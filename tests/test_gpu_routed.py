@@ -523,7 +523,7 @@ def test_refusals(k):
         lambda: k.matmul_i8_grouped(q, s, W, WS, r.offsets[:3].cpu()),
         lambda: k.sort_by_expert(torch.zeros(4, 2, **cuda), 3), lambda: k.sort_by_expert(r.position, 0), lambda: k.sort_by_expert(r.position, 65537),
         lambda: k.sort_by_expert(r.position.t(), 3), lambda: k.sort_by_expert(r.position.cpu(), 3), lambda: k.sort_by_expert(torch.zeros(2, 65, dtype=torch.int32, **cuda), 3),
-        lambda: k.dispatch(x[:3], r), lambda: k.dispatch(x.double(), r), lambda: k.dispatch(x, (r.order, r.position)), lambda: k.dispatch_i8(x[:2], r),
+        lambda: k.dispatch(x[:3], r), lambda: k.dispatch(x.double(), r), lambda: k.dispatch_i8(x[:2], r),
         lambda: k.dispatch_i8(q, r), lambda: k.combine(y[:7], w, r), lambda: k.combine(y, w[:3], r), lambda: k.combine(y, w.double(), r),
         lambda: k.combine(y.double(), w, r), lambda: k.combine(y, w.cpu(), r), lambda: k.combine(y, w.t().contiguous().t(), r),
         lambda: k.combine_backward(x, y.half(), w, r), lambda: k.combine_backward(x[:3], y, w, r), lambda: k.combine_backward(x, y[:, :4], w, r),
@@ -537,7 +537,17 @@ def test_refusals(k):
 
 def test_c_entries_refuse(k):
     """The library checks what the Python layer cannot be trusted to have checked, before anything is launched."""
+    import ctypes
+
     lib, h = k._lib, k.handle
+    i, l, z, v = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
+    lib.stlq_b200_quantize_rows.argtypes = [v, v, i, l, l, i, v, l, v, v]
+    lib.stlq_b200_matmul_i8.argtypes = [v, v, l, v, v, l, v, v, l, i, i, v, i, l, v]
+    lib.stlq_b200_matmul_i8_grouped.argtypes = [v, v, l, v, v, l, v, v, v, i, l, i, i, v, i, l, v]
+    lib.stlq_b200_sort_by_expert.argtypes = [v, v, i, l, i, i, v, v, v, v, z, v]
+    lib.stlq_b200_dispatch.argtypes = [v, v, i, l, l, i, i, v, v, i, v, l, v]
+    lib.stlq_b200_combine.argtypes = [v, v, i, l, l, i, i, v, i, v, v, i, v, l, v]
+    lib.stlq_b200_combine_backward.argtypes = [v, v, i, l, v, l, l, i, i, v, i, v, v, i, v, l, v, v]
     t = torch.zeros(4096, device="cuda")
     p = t.data_ptr()
     refused = [

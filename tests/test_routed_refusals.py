@@ -11,6 +11,15 @@ torch = pytest.importorskip("torch")
 
 def test_c_entries_reject_a_null_handle():
     lib = operators._ready()[0]
+    i, l, z, v = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
+    lib.stlq_b200_quantize_rows.argtypes = [v, v, i, l, l, i, v, l, v, v]
+    lib.stlq_b200_matmul_i8.argtypes = [v, v, l, v, v, l, v, v, l, i, i, v, i, l, v]
+    lib.stlq_b200_matmul_i8_grouped.argtypes = [v, v, l, v, v, l, v, v, v, i, l, i, i, v, i, l, v]
+    lib.stlq_b200_sort_by_expert.argtypes = [v, v, i, l, i, i, v, v, v, v, z, v]
+    lib.stlq_b200_dispatch.argtypes = [v, v, i, l, l, i, i, v, v, i, v, l, v]
+    lib.stlq_b200_dispatch_i8.argtypes = [v, v, i, l, l, i, i, v, v, i, v, l, v, v]
+    lib.stlq_b200_combine.argtypes = [v, v, i, l, l, i, i, v, i, v, v, i, v, l, v]
+    lib.stlq_b200_combine_backward.argtypes = [v, v, i, l, v, l, l, i, i, v, i, v, v, i, v, l, v, v]
     calls = [
         lambda: lib.stlq_b200_quantize_rows(None, None, 0, 8, 4, 8, None, 16, None, None),
         lambda: lib.stlq_b200_matmul_i8(None, None, 16, None, None, 16, None, None, 4, 4, 16, None, 0, 4, None),
@@ -31,6 +40,7 @@ def test_c_entries_reject_a_null_handle():
                                                     (1, 0, 4, 1), (1, 65, 4, 1), (-1, 1, 4, 1), (1 << 31, 1, 4, 1), (1 << 30, 2, 4, 1)])
 def test_sort_workspace(tokens, topk, experts, rc):
     lib = operators._ready()[0]
+    lib.stlq_b200_sort_by_expert_workspace.argtypes = [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]
     size = ctypes.c_size_t(7)
     assert lib.stlq_b200_sort_by_expert_workspace(tokens, topk, experts, ctypes.byref(size)) == rc
     assert (size.value == 0) if rc or tokens == 0 else (0 < size.value < (1 << 31))
