@@ -23,7 +23,9 @@ namespace {
 
 using stlq_b200::Ck;
 using stlq_b200::DeviceScope;
+using stlq_b200::LetLaterStart;
 using stlq_b200::SetError;
+using stlq_b200::WaitForEarlier;
 namespace tc = stlq_b200::tc;
 
 constexpr int kChannels = 128;                       // channels of a CTA's tile (its share of the MMA's M)
@@ -164,6 +166,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (kMode == kPair) tc::TmemAllocPair(tmem_slot, S::kTmem);
         else tc::TmemAlloc(tmem_slot, S::kTmem);
     }
+    LetLaterStart();
+    WaitForEarlier();
     if (a.offsets) {
         for (int e = threadIdx.x; e < a.experts; e += kThreads) sg.end[e] = min(max(a.offsets[e + 1], 0), a.rows);
         __syncthreads();
@@ -470,6 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Without a term to sum (kdim 0): the bias, and zeros after the last segment.
 template <typename T>
 __global__ void BiasRowsKernel(const MatmulArgs a) {
+    LetLaterStart();
+    WaitForEarlier();
     const int64_t total = static_cast<int64_t>(a.rows) * a.n;
     const int kept = a.offsets ? min(max(a.offsets[a.experts], 0), a.rows) : a.rows;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
@@ -566,11 +572,13 @@ cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = smem;
     config.stream = o.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
     config.attrs = attr;
-    config.numAttrs = kMode == kOne ? 0 : 1;
+    config.numAttrs = kMode == kOne ? 1 : 2;
     return cudaLaunchKernelEx(&config, kernel, tw, tx, to, a, cluster);
 }
 
@@ -600,8 +608,7 @@ cudaError_t LaunchAs(const Operands& o, const MatmulArgs& a, Mode mode, int heig
 template <typename T>
 cudaError_t Launch(const Operands& o, const MatmulArgs& a) {
     if (a.kdim == 0) {
-        BiasRowsKernel<T><<<o.sms * 4, 256, 0, o.stream>>>(a);
-        return cudaGetLastError();
+        return stlq_b200::LaunchAfter(BiasRowsKernel<T>, o.sms * 4, 256, 0, o.stream, a);
     }
     const int64_t ct = (a.n + kChannels - 1) / kChannels;
     const int nk = (a.kdim + kTileK - 1) / kTileK;

@@ -57,6 +57,31 @@ private:
     bool ok_ = false, restore_ = false;
 };
 
+#ifdef __CUDACC__
+// Programmatic dependent launch: a kernel launched with LaunchAfter may start while the one before it
+// in the stream ends.  Each such kernel calls WaitForEarlier before it touches global memory; that
+// returns when everything launched earlier in the stream has finished and is visible (each of these
+// kernels waits for the one before it), so the results are those of launches one after the other.
+// LetLaterStart allows the next one to come up, which it does once every block has called it or left.
+__device__ __forceinline__ void WaitForEarlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void LetLaterStart() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+template <typename... P, typename... A>
+cudaError_t LaunchAfter(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(block);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, P(args)...);
+}
+#endif
+
 }  // namespace stlq_b200
 
 struct stlq_b200_kernels {

@@ -21,7 +21,10 @@ namespace {
 
 using stlq_b200::Ck;
 using stlq_b200::DeviceScope;
+using stlq_b200::LaunchAfter;
+using stlq_b200::LetLaterStart;
 using stlq_b200::SetError;
+using stlq_b200::WaitForEarlier;
 
 constexpr int kBlock = 256;
 
@@ -68,6 +71,47 @@ __device__ __forceinline__ int Quantise(float x, float amax, float down) {
     return __float2int_rn(__fdiv_rn(__fmul_rn(__fmul_rn(x, down), 127.0f), __fmul_rn(amax, down)));
 }
 
+// The same for N values, mostly without a division, which bound the kernel (16,384 x 4,096 bfloat16: 90 us
+// with one for each value): x r with r = 127 / amax differs from the quotient by less than 4 roundings of a
+// number up to 127 (4 * 127 * 2^-24 < 3.1e-5), so it rounds to the same integer unless it is nearer than that
+// to the middle between two; a pack with such a value is divided.  Adding 1.5 * 2^23 rounds to an integer and
+// leaves it in the low bits.  r is infinite or NaN where amax is too small for it (or the row has none): divided.
+template <typename T, int N>
+__device__ __forceinline__ Pack<int8_t, N> QuantisePack(const Pack<T, N>& x, float amax, float r, float down) {
+    constexpr float kMagic = 12582912.0f;
+    Pack<int8_t, N> q;
+    bool sure = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float v = ToFloat(x.v[i]);
+        const float t = fmaf(v, r, kMagic);
+        sure = sure && fabsf(fmaf(v, r, kMagic - t)) < 0.5f - 4e-5f;
+        q.v[i] = static_cast<int8_t>(__float_as_int(t));
+    }
+    if (!sure) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q.v[i] = static_cast<int8_t>(Quantise(ToFloat(x.v[i]), amax, down));
+    }
+    return q;
+}
+
+// The larger of `top` and the |x|, by bits: unsigned order puts every NaN above infinity above the numbers.
+template <typename T, int N>
+__device__ __forceinline__ unsigned int LargestBits(const Pack<T, N>& x, unsigned int top) {
+    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+        using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+        const T2* p = reinterpret_cast<const T2*>(&x);
+        T2 m = __habs2(p[0]);
+#pragma unroll
+        for (int i = 1; i < N / 2; ++i) m = __hmax2_nan(m, __habs2(p[i]));
+        return max(top, max(__float_as_uint(fabsf(ToFloat(m.x))), __float_as_uint(fabsf(ToFloat(m.y)))));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(ToFloat(x.v[i])) & 0x7fffffffu);
+        return top;
+    }
+}
+
 // One group of L threads quantises one row and writes it once (position null) or to the rows of its
 // choices.  The row is read once: a thread keeps its first kHold vectors in registers between the
 // maximum and the rounding, and re-reads the rest.
@@ -86,21 +130,19 @@ __global__ void __launch_bounds__(kBlock)
     const int full = cols / N;
     const T* xr = x + (real ? row : 0) * ldx;
     Pack<T, N> hold[kHold];
-    // The largest |x| by its bits: unsigned order puts every NaN above infinity above the numbers.
     unsigned int top = 0;
+    LetLaterStart();
+    WaitForEarlier();
     if (real) {
 #pragma unroll
         for (int h = 0; h < kHold; ++h) {
             const int c = at + h * L;
             if (c >= full) break;
             hold[h] = *reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N);
-#pragma unroll
-            for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(ToFloat(hold[h].v[i])) & 0x7fffffffu);
+            top = LargestBits(hold[h], top);
         }
         for (int c = at + kHold * L; c < full; c += L) {
-            const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N);
-#pragma unroll
-            for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(ToFloat(v.v[i])) & 0x7fffffffu);
+            top = LargestBits(*reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N), top);
         }
         for (int c = full * N + at; c < cols; c += L) top = max(top, __float_as_uint(ToFloat(xr[c])) & 0x7fffffffu);
     }
@@ -116,6 +158,7 @@ __global__ void __launch_bounds__(kBlock)
     const bool finite = top < 0x7f800000u;
     const bool some = finite && top != 0;
     const float down = amax > 1e36f ? 0.00390625f : 1.0f;
+    const float inverse = __fdiv_rn(127.0f, amax);
     const float s = finite ? __fdiv_rn(amax, 127.0f) : __int_as_float(0x7fc00000);
     const int kept = position ? Kept(offsets, experts, pairs) : 0;
     const int copies = position ? topk : 1;
@@ -126,12 +169,8 @@ __global__ void __launch_bounds__(kBlock)
     };
     // Dropped choices get a row of zeros with scale 0.
     auto store = [&](int c, const Pack<T, N>& v) {
-        Pack<int8_t, N> r, zero;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            r.v[i] = some ? static_cast<int8_t>(Quantise(ToFloat(v.v[i]), amax, down)) : static_cast<int8_t>(0);
-            zero.v[i] = 0;
-        }
+        Pack<int8_t, N> r{}, zero{};
+        if (some) r = QuantisePack(v, amax, inverse, down);
         for (int j = 0; j < copies; ++j) {
             const int64_t to = target(j);
             if (to >= 0)
@@ -162,15 +201,19 @@ __global__ void __launch_bounds__(kBlock)
 
 // ---- sort by expert ----------------------------------------------------------------------------
 
-// A counting sort over `bins` digits, stable: a tile of kTile keys per block, each of its warps
-// ranking a contiguous piece 32 keys at a time (__match_any_sync gives the lanes that share a
-// digit).  Up to kOneBins - 1 experts it is one pass; above that two passes of half the key's bits
-// each, from the low digit to the high one.
+// A counting sort over `bins` digits, stable: a tile of keys per block, each of its warps ranking a
+// contiguous piece 32 keys at a time (__match_any_sync gives the lanes that share a digit).  Up to
+// kOneBins - 1 experts it is one pass; above that two passes of half the key's bits each, from the low
+// digit to the high one.  A sort that fits one block is one launch; others take three a pass: count, scan
+// each digit over the tiles, scatter.
 constexpr int kSortBlock = 512;
 constexpr int kSortWarps = kSortBlock / 32;
 constexpr int kPerWarp = 256;
 constexpr int kTile = kSortWarps * kPerWarp;
 constexpr int kOneBins = 1025;
+constexpr int kAloneBlock = 1024;
+constexpr int kAloneRounds = 16;                         // keys of a lane
+constexpr int kAlone = kAloneBlock * kAloneRounds;       // the most pairs of a sort by one block
 
 struct SortPass {
     const void* ids;   // first pass: the caller's ids
@@ -186,129 +229,243 @@ __device__ __forceinline__ int KeyOf(const SortPass& a, int i) {
     return id >= 0 && id < a.experts ? static_cast<int>(id) : a.experts;
 }
 
-// Digits of this warp's keys counted into count[bins]; kRank: each key's rank among the warp's keys
-// of its digit goes to rank[].
-template <bool kRank>
-__device__ __forceinline__ void CountWarp(const SortPass& a, int first, unsigned short* count, unsigned short* rank) {
+// One round of a warp: each lane's digit (bins: no key) counted into count[]; the lane's rank among the
+// warp's keys of its digit so far.
+__device__ __forceinline__ int CountRound(int d, int bins, unsigned short* count) {
     const int lane = threadIdx.x & 31;
-    for (int r = 0; r < kPerWarp / 32; ++r) {
-        const int i = first + r * 32 + lane;
-        const int d = i < a.n ? (KeyOf(a, i) >> a.shift) & a.mask : a.bins;  // no key: a digit of its own
-        const unsigned same = __match_any_sync(0xffffffffu, d);
-        const int before = d < a.bins ? count[d] : 0;
-        const int mine = __popc(same & ((1u << lane) - 1));
-        if (kRank) rank[r] = static_cast<unsigned short>(before + mine);
-        __syncwarp();
-        if (mine == 0 && d < a.bins) count[d] = static_cast<unsigned short>(before + __popc(same));
-        __syncwarp();
+    const unsigned same = __match_any_sync(0xffffffffu, d);
+    const int before = d < bins ? count[d] : 0;
+    const int mine = __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (mine == 0 && d < bins) count[d] = static_cast<unsigned short>(before + __popc(same));
+    __syncwarp();
+    return before + mine;
+}
+
+// The sum of x over the threads before this one in its block; `all`: over all.
+__device__ __forceinline__ int ScanThreads(int x, int* part, int* all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int s = x;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+    }
+    if (lane == 31) part[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+        int t = lane < warps ? part[lane] : 0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += y;
+        }
+        part[lane] = t;
+    }
+    __syncthreads();
+    *all = part[warps - 1];
+    const int before = (warp ? part[warp - 1] : 0) + s - x;
+    __syncthreads();
+    return before;
+}
+
+// counts [warps][bins] to the sums over the warps before; base[b] = the sum over the digits before b
+// of `sum(b, own)`, where own is the digit's count in this block.
+template <typename F>
+__device__ __forceinline__ void ScanDigits(unsigned short* counts, int warps, int bins, int* base, F&& sum) {
+    __shared__ int part[32];
+    int carry = 0;
+    for (int b0 = 0; b0 < bins; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        int own = 0;
+        if (b < bins)
+            for (int w = 0; w < warps; ++w) {
+                const int c = counts[w * bins + b];
+                counts[w * bins + b] = static_cast<unsigned short>(own);
+                own += c;
+            }
+        int all;
+        const int before = ScanThreads(b < bins ? sum(b, own) : 0, part, &all);
+        if (b < bins) base[b] = carry + before;
+        carry += all;
+    }
+    __syncthreads();
+}
+
+// The whole sort in one block.
+__global__ void __launch_bounds__(kAloneBlock)
+    SortAloneKernel(SortPass a, int rounds, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
+    extern __shared__ int base[];  // [bins], then the counts [warps][bins]
+    unsigned short* counts = reinterpret_cast<unsigned short*>(base + a.bins);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    LetLaterStart();
+    for (int i = threadIdx.x; i < warps * a.bins; i += blockDim.x) counts[i] = 0;
+    __syncthreads();
+    WaitForEarlier();
+    const int first = warp * rounds * 32 + lane;
+    int key[kAloneRounds];
+    unsigned short rank[kAloneRounds];
+#pragma unroll
+    for (int r = 0; r < kAloneRounds; ++r)
+        if (r < rounds) key[r] = first + r * 32 < a.n ? KeyOf(a, first + r * 32) : a.bins;
+#pragma unroll
+    for (int r = 0; r < kAloneRounds; ++r)
+        if (r < rounds) rank[r] = static_cast<unsigned short>(CountRound(key[r], a.bins, counts + warp * a.bins));
+    __syncthreads();
+    ScanDigits(counts, warps, a.bins, base, [](int, int own) { return own; });
+    for (int b = threadIdx.x; b < a.bins; b += blockDim.x) offsets[b] = base[b];
+#pragma unroll
+    for (int r = 0; r < kAloneRounds; ++r) {
+        const int i = first + r * 32;
+        if (r < rounds && i < a.n) {
+            const int to = base[key[r]] + counts[warp * a.bins + key[r]] + rank[r];
+            order[to] = i;
+            position[i] = to;
+        }
     }
 }
 
+// hist[b * tiles + tile] = keys of digit b in the tile.
 __global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* __restrict__ hist, int* __restrict__ totals) {
     extern __shared__ unsigned short counts[];  // [kSortWarps][bins]
+    LetLaterStart();
     for (int i = threadIdx.x; i < kSortWarps * a.bins; i += kSortBlock) counts[i] = 0;
     __syncthreads();
-    const int warp = threadIdx.x >> 5;
-    CountWarp<false>(a, blockIdx.x * kTile + warp * kPerWarp, counts + warp * a.bins, nullptr);
+    WaitForEarlier();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int first = blockIdx.x * kTile + warp * kPerWarp + lane;
+    int key[kPerWarp / 32];
+#pragma unroll
+    for (int r = 0; r < kPerWarp / 32; ++r) key[r] = first + r * 32 < a.n ? KeyOf(a, first + r * 32) : -1;
+#pragma unroll
+    for (int r = 0; r < kPerWarp / 32; ++r) CountRound(key[r] < 0 ? a.bins : (key[r] >> a.shift) & a.mask, a.bins, counts + warp * a.bins);
     __syncthreads();
     for (int b = threadIdx.x; b < a.bins; b += kSortBlock) {
         int sum = 0;
+#pragma unroll
         for (int w = 0; w < kSortWarps; ++w) sum += counts[w * a.bins + b];
         hist[static_cast<int64_t>(b) * a.tiles + blockIdx.x] = sum;
     }
     if (totals)  // two-pass sorts: keys per expert (whole numbers, so the order of the additions is free)
-        for (int i = blockIdx.x * kTile + threadIdx.x; i < min(a.n, (static_cast<int>(blockIdx.x) + 1) * kTile); i += kSortBlock)
-            atomicAdd(totals + KeyOf(a, i), 1);
+#pragma unroll
+        for (int r = 0; r < kPerWarp / 32; ++r) {
+            const unsigned same = __match_any_sync(0xffffffffu, key[r]);
+            if (key[r] >= 0 && (same & ((1u << lane) - 1)) == 0) atomicAdd(totals + key[r], __popc(same));
+        }
 }
 
-// Exclusive scan of n counters by one block.
-__device__ void ScanBlock(int* v, int64_t n) {
+// One warp per digit: its counts to the sums over the tiles before, its total to sums[].  The block after
+// the digits' (two-pass sorts) scans the keys per expert in place.
+constexpr int kScanBlock = 1024;
+__global__ void __launch_bounds__(kScanBlock)
+    SortScanKernel(int* __restrict__ hist, int bins, int tiles, int* __restrict__ sums, int* __restrict__ totals, int experts) {
     __shared__ int part[32];
-    __shared__ int carry;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if (threadIdx.x == 0) carry = 0;
-    __syncthreads();
-    for (int64_t base = 0; base < n; base += blockDim.x) {
-        const int64_t i = base + threadIdx.x;
-        const int x = i < n ? v[i] : 0;
-        int s = x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    LetLaterStart();
+    WaitForEarlier();
+    if (totals && blockIdx.x == gridDim.x - 1) {
+        constexpr int kEach = 8;
+        int carry = 0;
+        for (int e0 = 0; e0 < experts; e0 += kScanBlock * kEach) {
+            const int e = e0 + threadIdx.x * kEach;
+            int v[kEach], own = 0, all;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) v[i] = e + i < experts ? totals[e + i] : 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) own += v[i];
+            int before = carry + ScanThreads(own, part, &all);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                if (e + i < experts) totals[e + i] = before;
+                before += v[i];
+            }
+            carry += all;
+        }
+        if (threadIdx.x == 0) totals[experts] = carry;  // rows kept: the dropped pairs' count gives way
+        return;
+    }
+    const int b = blockIdx.x * (kScanBlock / 32) + warp;
+    if (b >= bins) return;
+    int* own = hist + static_cast<int64_t>(b) * tiles;
+    int carry = 0;
+    for (int t0 = 0; t0 < tiles; t0 += 128) {
+        int v[4], s = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = t0 + lane * 4 + i < tiles ? own[t0 + lane * 4 + i] : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += v[i];
+        const int mine = s;
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += y;
         }
-        if (lane == 31) part[warp] = s;
-        __syncthreads();
-        if (warp == 0) {
-            int t = lane < warps ? part[lane] : 0;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, t, o);
-                if (lane >= o) t += y;
-            }
-            part[lane] = t;
+        int before = carry + s - mine;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (t0 + lane * 4 + i < tiles) own[t0 + lane * 4 + i] = before;
+            before += v[i];
         }
-        __syncthreads();
-        const int before = carry + (warp ? part[warp - 1] : 0);
-        if (i < n) v[i] = before + s - x;
-        const int all = part[warps - 1];
-        __syncthreads();
-        if (threadIdx.x == 0) carry += all;
-        __syncthreads();
+        carry += __shfl_sync(0xffffffffu, s, 31);
     }
+    if (lane == 0) sums[b] = carry;
 }
 
-// Block 0 scans the counters of a pass; block 1, when there is one, the keys per expert.
-__global__ void __launch_bounds__(1024) SortScanKernel(int* __restrict__ hist, int64_t n, int* __restrict__ totals, int64_t m) {
-    if (blockIdx.x == 0) ScanBlock(hist, n);
-    else ScanBlock(totals, m);
-}
-
-// offsets (one-pass sorts) are the counters of each digit's first tile.
+// Each key to its place.  offsets (one-pass sorts): where each digit begins.
 __global__ void __launch_bounds__(kSortBlock)
-    SortScatterKernel(SortPass a, const int* __restrict__ hist, int* __restrict__ keys_out, int* __restrict__ pairs_out,
-                      int* __restrict__ position, int* __restrict__ offsets) {
-    extern __shared__ unsigned short counts[];  // [kSortWarps][bins], then [bins] ints
-    int* base = reinterpret_cast<int*>(counts + ((kSortWarps * a.bins + 1) & ~1));
+    SortScatterKernel(SortPass a, const int* __restrict__ hist, const int* __restrict__ sums, int* __restrict__ keys_out,
+                      int* __restrict__ pairs_out, int* __restrict__ position, int* __restrict__ offsets) {
+    extern __shared__ int base[];  // [bins], then the counts [kSortWarps][bins]
+    unsigned short* counts = reinterpret_cast<unsigned short*>(base + a.bins);
+    LetLaterStart();
     for (int i = threadIdx.x; i < kSortWarps * a.bins; i += kSortBlock) counts[i] = 0;
     __syncthreads();
+    WaitForEarlier();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int first = blockIdx.x * kTile + warp * kPerWarp;
+    const int first = blockIdx.x * kTile + warp * kPerWarp + lane;
+    int key[kPerWarp / 32], pair[kPerWarp / 32];
     unsigned short rank[kPerWarp / 32];
-    CountWarp<true>(a, first, counts + warp * a.bins, rank);
-    __syncthreads();
-    for (int b = threadIdx.x; b < a.bins; b += kSortBlock) {
-        int sum = 0;
-        for (int w = 0; w < kSortWarps; ++w) {
-            const int c = counts[w * a.bins + b];
-            counts[w * a.bins + b] = static_cast<unsigned short>(sum);
-            sum += c;
-        }
-        base[b] = hist[static_cast<int64_t>(b) * a.tiles + blockIdx.x];
-        if (offsets && blockIdx.x == 0) offsets[b] = base[b];
-    }
-    __syncthreads();
+#pragma unroll
     for (int r = 0; r < kPerWarp / 32; ++r) {
-        const int i = first + r * 32 + lane;
-        if (i >= a.n) break;
-        const int key = KeyOf(a, i), d = (key >> a.shift) & a.mask;
+        const int i = first + r * 32;
+        key[r] = i < a.n ? KeyOf(a, i) : -1;
+        pair[r] = i < a.n && a.pairs ? a.pairs[i] : i;
+    }
+#pragma unroll
+    for (int r = 0; r < kPerWarp / 32; ++r)
+        rank[r] = static_cast<unsigned short>(
+            CountRound(key[r] < 0 ? a.bins : (key[r] >> a.shift) & a.mask, a.bins, counts + warp * a.bins));
+    __syncthreads();
+    ScanDigits(counts, kSortWarps, a.bins, base, [&](int b, int) { return sums[b]; });
+    if (offsets && blockIdx.x == 0)
+        for (int b = threadIdx.x; b < a.bins; b += kSortBlock) offsets[b] = base[b];
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.bins; b += kSortBlock) base[b] += hist[static_cast<int64_t>(b) * a.tiles + blockIdx.x];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kPerWarp / 32; ++r) {
+        if (key[r] < 0) continue;
+        const int d = (key[r] >> a.shift) & a.mask;
         const int to = base[d] + counts[warp * a.bins + d] + rank[r];
-        const int pair = a.pairs ? a.pairs[i] : i;
-        pairs_out[to] = pair;
-        if (keys_out) keys_out[to] = key;
-        if (position) position[pair] = to;
+        pairs_out[to] = pair[r];
+        if (keys_out) keys_out[to] = key[r];
+        if (position) position[pair[r]] = to;
     }
 }
 
-__global__ void NoPairsKernel(int* offsets, int n) {
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) offsets[i] = 0;
+__global__ void ZeroKernel(int* p, int n) {
+    LetLaterStart();
+    WaitForEarlier();
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) p[i] = 0;
 }
 
 struct SortPlan {
     int bins[2], shift[2], passes, tiles;
-    size_t hist, keys, pairs, totals, bytes;  // places in the workspace
+    size_t sums, keys, pairs, bytes;  // places in the workspace, which begins with the counts of each tile
 };
+
+bool Alone(int64_t n, int experts) { return n <= kAlone && experts + 1 <= kOneBins; }
 
 SortPlan PlanSort(int64_t n, int experts) {
     SortPlan p{};
+    if (Alone(n, experts)) return p;
     p.tiles = static_cast<int>((n + kTile - 1) / kTile);
     if (experts + 1 <= kOneBins) {
         p.passes = 1;
@@ -323,19 +480,17 @@ SortPlan PlanSort(int64_t n, int experts) {
     }
     const auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     const size_t most = std::max(p.bins[0], p.bins[1]);
-    p.keys = up(most * p.tiles * sizeof(int));
-    p.pairs = p.keys;
-    p.totals = p.keys;
-    p.bytes = p.keys;
+    p.sums = up(most * p.tiles * sizeof(int));
+    p.keys = p.sums + up(most * sizeof(int));
+    p.pairs = p.bytes = p.keys;
     if (p.passes == 2) {
         p.pairs = p.keys + up(static_cast<size_t>(n) * sizeof(int));
-        p.totals = p.pairs + up(static_cast<size_t>(n) * sizeof(int));
-        p.bytes = p.totals;
+        p.bytes = p.pairs + up(static_cast<size_t>(n) * sizeof(int));
     }
     return p;
 }
 
-size_t SortSmem(int bins) { return ((static_cast<size_t>(kSortWarps) * bins + 1) & ~static_cast<size_t>(1)) * 2 + bins * 4; }
+size_t SortSmem(int warps, int bins) { return static_cast<size_t>(bins) * 4 + static_cast<size_t>(warps) * bins * 2; }
 
 // ---- exchange ----------------------------------------------------------------------------------
 
@@ -347,6 +502,8 @@ __global__ void __launch_bounds__(kBlock)
                    const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
                    unsigned char* __restrict__ out, int64_t ldo) {
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + threadIdx.x / L;
+    LetLaterStart();
+    WaitForEarlier();
     if (t >= tokens) return;
     const int kept = Kept(offsets, experts, pairs);
     const V* row = reinterpret_cast<const V*>(x + t * ldx);
@@ -368,6 +525,8 @@ __global__ void __launch_bounds__(kBlock)
                   const void* __restrict__ weights, int wtype, const int* __restrict__ position,
                   const int* __restrict__ offsets, int experts, int pairs, T* __restrict__ out, int64_t ldo) {
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + threadIdx.x / L;
+    LetLaterStart();
+    WaitForEarlier();
     if (t >= tokens) return;
     const unsigned kept = static_cast<unsigned>(Kept(offsets, experts, pairs));
     const int full = cols / N;
@@ -413,6 +572,8 @@ __global__ void __launch_bounds__(kBlock)
     const int group = threadIdx.x / L, at = threadIdx.x % L, warp = threadIdx.x >> 5;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + group;
     const bool real = t < tokens;
+    LetLaterStart();
+    WaitForEarlier();
     const int kept = Kept(offsets, experts, pairs);
     const int full = cols / N;
     const T* d = dout + (real ? t : 0) * ldd;
@@ -511,6 +672,7 @@ int Quantize(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int6
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int pairs = position ? static_cast<int>(rows * topk) : 0;
     bool fits = true;
+    cudaError_t error = cudaSuccess;
     ForType(x_dtype, [&](auto one) {
         using T = decltype(one);
         constexpr int N = 16 / sizeof(T);
@@ -522,15 +684,15 @@ int Quantize(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int6
             fits = grid != 0;
             if (!fits) return;
             if (wide)
-                QuantizeRowsKernel<T, N, L><<<grid, kBlock, 0, s>>>(xp, ldx, rows, cols, topk, position, offsets, experts,
+                error = LaunchAfter(QuantizeRowsKernel<T, N, L>, grid, kBlock, 0, s, xp, ldx, rows, cols, topk, position, offsets, experts,
                                                                     pairs, q, ldq, scale);
             else
-                QuantizeRowsKernel<T, 1, L><<<grid, kBlock, 0, s>>>(xp, ldx, rows, cols, topk, position, offsets, experts,
+                error = LaunchAfter(QuantizeRowsKernel<T, 1, L>, grid, kBlock, 0, s, xp, ldx, rows, cols, topk, position, offsets, experts,
                                                                     pairs, q, ldq, scale);
         });
     });
     if (!fits) return Bad("too many rows");
-    return Ck(cudaGetLastError(), "quantize_rows");
+    return Ck(error, "quantize_rows");
 }
 
 }  // namespace
@@ -582,33 +744,37 @@ int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtyp
         DeviceScope scope(k->device);
         if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (n == 0) {
-            NoPairsKernel<<<std::min(experts / 256 + 1, 64), 256, 0, s>>>(offsets, experts + 1);
-            return Ck(cudaGetLastError(), "sort_by_expert");
+        if (n == 0) return Ck(LaunchAfter(ZeroKernel, std::min(experts / 256 + 1, 64), 256, 0, s, offsets, experts + 1), "sort_by_expert");
+        SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, nullptr, n, experts, 0, 0x7fffffff, experts + 1, p.tiles};
+        const size_t most = 72 << 10;
+        if (Alone(n, experts)) {
+            if (int rc = Ck(cudaFuncSetAttribute(SortAloneKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
+            // As many warps as there are rounds for, so that few pairs take one round.
+            const int warps = std::min(kAloneBlock / 32, (n + 31) / 32);
+            const int rounds = (n + warps * 32 - 1) / (warps * 32);
+            return Ck(LaunchAfter(SortAloneKernel, 1, warps * 32, SortSmem(warps, a.bins), s, a, rounds, order, position, offsets), "sort_by_expert");
         }
         char* ws = static_cast<char*>(workspace);
         int* hist = reinterpret_cast<int*>(ws);
+        int* sums = reinterpret_cast<int*>(ws + p.sums);
         int* keys = reinterpret_cast<int*>(ws + p.keys);
         int* pairs = reinterpret_cast<int*>(ws + p.pairs);
-        if (int rc = Ck(cudaFuncSetAttribute(SortScatterKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10), "sort_by_expert")) return rc;
-        if (int rc = Ck(cudaFuncSetAttribute(SortCountKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10), "sort_by_expert")) return rc;
-        SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, nullptr, n, experts, 0, 0x7fffffff, p.bins[0], p.tiles};
-        if (p.passes == 1) {
-            SortCountKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, nullptr);
-            SortScanKernel<<<1, 1024, 0, s>>>(hist, static_cast<int64_t>(a.bins) * p.tiles, nullptr, 0);
-            SortScatterKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, nullptr, order, position, offsets);
-            return Ck(cudaGetLastError(), "sort_by_expert");
-        }
-        if (int rc = Ck(cudaMemsetAsync(offsets, 0, sizeof(int) * (static_cast<size_t>(experts) + 1), s), "sort_by_expert")) return rc;
+        if (int rc = Ck(cudaFuncSetAttribute(SortScatterKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
+        if (int rc = Ck(cudaFuncSetAttribute(SortCountKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
+        const auto pass = [&](const SortPass& x, int* totals, int* keys_out, int* pairs_out, int* position_out, int* offsets_out) {
+            const size_t smem = SortSmem(kSortWarps, x.bins);
+            const int digits = (x.bins + kScanBlock / 32 - 1) / (kScanBlock / 32);
+            if (int rc = Ck(LaunchAfter(SortCountKernel, p.tiles, kSortBlock, smem, s, x, hist, totals), "sort_by_expert")) return rc;
+            if (int rc = Ck(LaunchAfter(SortScanKernel, digits + (totals ? 1 : 0), kScanBlock, 0, s, hist, x.bins, p.tiles, sums, totals, experts), "sort_by_expert")) return rc;
+            return Ck(LaunchAfter(SortScatterKernel, p.tiles, kSortBlock, smem, s, x, hist, sums, keys_out, pairs_out, position_out, offsets_out), "sort_by_expert");
+        };
+        if (p.passes == 1) return pass(a, nullptr, nullptr, order, position, offsets);
+        if (int rc = Ck(LaunchAfter(ZeroKernel, std::min(experts / 256 + 1, 64), 256, 0, s, offsets, experts + 1), "sort_by_expert")) return rc;
         a.mask = p.bins[0] - 1;
-        SortCountKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, offsets);
-        SortScanKernel<<<2, 1024, 0, s>>>(hist, static_cast<int64_t>(a.bins) * p.tiles, offsets, experts + 1);
-        SortScatterKernel<<<p.tiles, kSortBlock, SortSmem(a.bins), s>>>(a, hist, keys, pairs, nullptr, nullptr);
-        SortPass b{nullptr, 0, keys, pairs, n, experts, p.shift[1], 0x7fffffff, p.bins[1], p.tiles};
-        SortCountKernel<<<p.tiles, kSortBlock, SortSmem(b.bins), s>>>(b, hist, nullptr);
-        SortScanKernel<<<1, 1024, 0, s>>>(hist, static_cast<int64_t>(b.bins) * p.tiles, nullptr, 0);
-        SortScatterKernel<<<p.tiles, kSortBlock, SortSmem(b.bins), s>>>(b, hist, nullptr, order, position, nullptr);
-        return Ck(cudaGetLastError(), "sort_by_expert");
+        a.bins = p.bins[0];
+        if (int rc = pass(a, offsets, keys, pairs, nullptr, nullptr)) return rc;
+        const SortPass b{nullptr, 0, keys, pairs, n, experts, p.shift[1], 0x7fffffff, p.bins[1], p.tiles};
+        return pass(b, nullptr, nullptr, order, position, nullptr);
     });
 }
 
@@ -630,6 +796,7 @@ int stlq_b200_dispatch(stlq_b200_kernels* k, const void* x, int elem_bytes, int6
         const int bytes = cols * elem_bytes;
         const int64_t bx = ldx * elem_bytes, bo = ldo * elem_bytes;
         bool fits = true;
+        cudaError_t error = cudaSuccess;
         auto launch = [&](auto pack) {
             using V = decltype(pack);
             const int packs = bytes / static_cast<int>(sizeof(V));
@@ -638,7 +805,7 @@ int stlq_b200_dispatch(stlq_b200_kernels* k, const void* x, int elem_bytes, int6
                 const unsigned grid = Blocks(tokens, L);
                 fits = grid != 0;
                 if (!fits) return;
-                DispatchKernel<V, L><<<grid, kBlock, 0, s>>>(static_cast<const unsigned char*>(x), bx, tokens, packs, topk,
+                error = LaunchAfter(DispatchKernel<V, L>, grid, kBlock, 0, s, static_cast<const unsigned char*>(x), bx, tokens, packs, topk,
                                                              position, offsets, experts, pairs,
                                                              static_cast<unsigned char*>(out), bo);
             });
@@ -651,7 +818,7 @@ int stlq_b200_dispatch(stlq_b200_kernels* k, const void* x, int elem_bytes, int6
         else if (fit(2)) launch(uint16_t{});
         else launch(uint8_t{});
         if (!fits) return Bad("too many tokens");
-        return Ck(cudaGetLastError(), "dispatch");
+        return Ck(error, "dispatch");
     });
 }
 
@@ -672,6 +839,7 @@ int stlq_b200_combine(stlq_b200_kernels* k, const void* y, int dtype, int64_t ld
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const int pairs = static_cast<int>(tokens * topk);
         bool fits = true;
+        cudaError_t error = cudaSuccess;
         ForType(dtype, [&](auto one) {
             using T = decltype(one);
             constexpr int N = 16 / sizeof(T);
@@ -684,15 +852,15 @@ int stlq_b200_combine(stlq_b200_kernels* k, const void* y, int dtype, int64_t ld
                 const T* yp = static_cast<const T*>(y);
                 T* op = static_cast<T*>(out);
                 if (wide)
-                    CombineKernel<T, N, L><<<grid, kBlock, 0, s>>>(yp, ldy, tokens, cols, topk, weights, weights_dtype,
+                    error = LaunchAfter(CombineKernel<T, N, L>, grid, kBlock, 0, s, yp, ldy, tokens, cols, topk, weights, weights_dtype,
                                                                    position, offsets, experts, pairs, op, ldo);
                 else
-                    CombineKernel<T, 1, L><<<grid, kBlock, 0, s>>>(yp, ldy, tokens, cols, topk, weights, weights_dtype,
+                    error = LaunchAfter(CombineKernel<T, 1, L>, grid, kBlock, 0, s, yp, ldy, tokens, cols, topk, weights, weights_dtype,
                                                                    position, offsets, experts, pairs, op, ldo);
             });
         });
         if (!fits) return Bad("too many tokens");
-        return Ck(cudaGetLastError(), "combine");
+        return Ck(error, "combine");
     });
 }
 
@@ -716,6 +884,7 @@ int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype
         const int pairs = static_cast<int>(tokens * topk);
         const size_t smem = sizeof(float) * (kBlock / 32) * topk;
         bool fits = true;
+        cudaError_t error = cudaSuccess;
         ForType(dtype, [&](auto one) {
             using T = decltype(one);
             constexpr int N = 16 / sizeof(T);
@@ -728,17 +897,17 @@ int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype
                 const T *dp = static_cast<const T*>(dout), *yp = static_cast<const T*>(y);
                 T* op = static_cast<T*>(dy);
                 if (wide)
-                    CombineBackwardKernel<T, N, L><<<grid, kBlock, smem, s>>>(dp, ldd, yp, ldy, tokens, cols, topk, weights,
+                    error = LaunchAfter(CombineBackwardKernel<T, N, L>, grid, kBlock, smem, s, dp, ldd, yp, ldy, tokens, cols, topk, weights,
                                                                               weights_dtype, position, offsets, experts,
                                                                               pairs, op, lddy, dweights);
                 else
-                    CombineBackwardKernel<T, 1, L><<<grid, kBlock, smem, s>>>(dp, ldd, yp, ldy, tokens, cols, topk, weights,
+                    error = LaunchAfter(CombineBackwardKernel<T, 1, L>, grid, kBlock, smem, s, dp, ldd, yp, ldy, tokens, cols, topk, weights,
                                                                               weights_dtype, position, offsets, experts,
                                                                               pairs, op, lddy, dweights);
             });
         });
         if (!fits) return Bad("too many tokens");
-        return Ck(cudaGetLastError(), "combine_backward");
+        return Ck(error, "combine_backward");
     });
 }
 

@@ -559,7 +559,7 @@ def test_c_entries_refuse(k):
         lib.stlq_b200_matmul_i8(h, p, 16, None, p, 16, p, None, 4, 4, 16, p, 0, 4, None), lib.stlq_b200_matmul_i8(h, p, 131072, p, p, 131072, p, None, 1, 1, 131072, p, 0, 1, None),
         lib.stlq_b200_matmul_i8_grouped(h, p, 16, p, p, 16, p, None, None, 2, 4, 4, 16, p, 0, 4, None),
         lib.stlq_b200_matmul_i8_grouped(h, p, 16, p, p, 16, p, None, p, 1025, 4, 4, 16, p, 0, 4, None),
-        lib.stlq_b200_sort_by_expert(h, p, 0, 4, 2, 3, p, p, p, p, 4096, None), lib.stlq_b200_sort_by_expert(h, p, 4, 4, 2, 3, p, p, p, p, 1, None),
+        lib.stlq_b200_sort_by_expert(h, p, 0, 4, 2, 3, p, p, p, p, 4096, None), lib.stlq_b200_sort_by_expert(h, p, 4, 40000, 2, 3, p, p, p, p, 1, None),
         lib.stlq_b200_sort_by_expert(h, p, 4, 2**31, 1, 3, p, p, p, p, 4096, None),
         lib.stlq_b200_dispatch(h, p, 8, 8, 4, 8, 2, p, p, 3, p, 8, None), lib.stlq_b200_dispatch(h, p, 4, 8, 4, 8, 65, p, p, 3, p, 8, None),
         lib.stlq_b200_dispatch(h, p, 4, 8, 4, 8, 2, None, p, 3, p, 8, None),
