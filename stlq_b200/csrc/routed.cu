@@ -67,32 +67,75 @@ __device__ __forceinline__ int Kept(const int* offsets, int experts, int pairs) 
 
 // 127 x / amax in 32 bits (two roundings), to the nearest integer, ties to even.  `down` keeps 127 x
 // finite for the largest rows: both are multiplied by 2^-8, which changes no bit of the quotient.
-__device__ __forceinline__ int Quantise(float x, float amax, float down) {
+__device__ __noinline__ int Quantise(float x, float amax, float down) {
     return __float2int_rn(__fdiv_rn(__fmul_rn(__fmul_rn(x, down), 127.0f), __fmul_rn(amax, down)));
 }
 
-// The same for N values, mostly without a division, which bound the kernel (16,384 x 4,096 bfloat16: 90 us
-// with one for each value): x r with r = 127 / amax differs from the quotient by less than 4 roundings of a
-// number up to 127 (4 * 127 * 2^-24 < 3.1e-5), so it rounds to the same integer unless it is nearer than that
-// to the middle between two; a pack with such a value is divided.  Adding 1.5 * 2^23 rounds to an integer and
-// leaves it in the low bits.  r is infinite or NaN where amax is too small for it (or the row has none): divided.
+// What a row's quantisation needs beside its largest |x|.
+struct RowScale {
+    float amax, down, r;
+    bool finite;
+    bool some;  // the row has numbers other than zeros, and nothing else
+    bool fast;  // 16-bit rows: products decide every value
+};
+
+// The same for N values without the division, which bound the kernel (16,384 x 4,096 bfloat16: 90 us with
+// one for each value).  Adding 1.5 * 2^23 rounds to an integer and leaves it in the low bits.
+//
+// 16-bit rows.  Write x = m 2^a and amax = M 2^b with integers below 2^11.  The quotient is exactly n + 1/2 only if
+// 254 m 2^s = (2n + 1) M for some s, and as 127 is prime, then 127 divides M or 2n + 1 = 127: but for the rows whose
+// M it divides (1 in 128, divided), the one tie is 63.5, which goes to 64.  Any other quotient v is at least
+// v / (254 m) > v 2^-19 from a tie.  So x r with r = (1 + 2^-20) 127 / amax, whose reciprocal and
+// product are off by less than 2^-21.4, is above v by 2^-20.8 to 2^-19.5 of it and rounds as the quotient does.
+//
+// 32-bit rows.  x r with r = 127 / amax differs from the rounded quotient by less than 4 roundings of a number up to
+// 127 (4 * 127 * 2^-24 < 3.1e-5), so it rounds to the same integer unless it is nearer than that to the middle
+// between two; a pack with such a value is divided, as are rows where r is infinite or NaN.
 template <typename T, int N>
-__device__ __forceinline__ Pack<int8_t, N> QuantisePack(const Pack<T, N>& x, float amax, float r, float down) {
+__device__ __forceinline__ Pack<int8_t, N> QuantisePack(const Pack<T, N>& x, const RowScale& s) {
     constexpr float kMagic = 12582912.0f;
-    Pack<int8_t, N> q;
+    unsigned low[N];
     bool sure = true;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float v = ToFloat(x.v[i]);
-        const float t = fmaf(v, r, kMagic);
-        sure = sure && fabsf(fmaf(v, r, kMagic - t)) < 0.5f - 4e-5f;
-        q.v[i] = static_cast<int8_t>(__float_as_int(t));
+        const float t = fmaf(v, s.r, kMagic);
+        if (sizeof(T) != 2) sure = sure && fabsf(fmaf(v, s.r, kMagic - t)) < 0.5f - 4e-5f;
+        low[i] = __float_as_uint(t);
     }
-    if (!sure) {
+    if (sizeof(T) == 2 ? !s.fast : !sure) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) q.v[i] = static_cast<int8_t>(Quantise(ToFloat(x.v[i]), amax, down));
+        for (int i = 0; i < N; ++i) low[i] = static_cast<unsigned>(Quantise(ToFloat(x.v[i]), s.amax, s.down));
+    }
+    Pack<int8_t, N> q;
+    if constexpr (N % 4 == 0) {
+        unsigned* w = reinterpret_cast<unsigned*>(&q);
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            w[i / 4] = __byte_perm(__byte_perm(low[i], low[i + 1], 0x0040), __byte_perm(low[i + 2], low[i + 3], 0x0040), 0x5410);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q.v[i] = static_cast<int8_t>(low[i]);
     }
     return q;
+}
+
+// From the bits of the largest |x| of a row.
+template <typename T>
+__device__ __forceinline__ RowScale ScaleOf(unsigned int top) {
+    RowScale s;
+    s.amax = __uint_as_float(top);
+    s.finite = top < 0x7f800000u;
+    s.some = s.finite && top != 0;
+    s.down = s.amax > 1e36f ? 0.00390625f : 1.0f;
+    s.fast = false;
+    if constexpr (sizeof(T) == 2) {
+        s.r = 127.0f * (1.0f + 9.5367431640625e-7f) * __fdividef(1.0f, s.amax);  // 1 + 2^-20
+        s.fast = s.amax >= 1e-30f && s.amax <= 1e30f && ((top & 0x7fffffu) | 0x800000u) % 127u != 0;
+    } else {
+        s.r = __fdiv_rn(127.0f, s.amax);
+    }
+    return s;
 }
 
 // The larger of `top` and the |x|, by bits: unsigned order puts every NaN above infinity above the numbers.
@@ -112,41 +155,51 @@ __device__ __forceinline__ unsigned int LargestBits(const Pack<T, N>& x, unsigne
     }
 }
 
-// One group of L threads quantises one row and writes it once (position null) or to the rows of its
-// choices.  The row is read once: a thread keeps its first kHold vectors in registers between the
-// maximum and the rounding, and re-reads the rest.
-constexpr int kHold = 4;
-
-template <typename T, int N, int L>
+// One group of L threads quantises one row and writes it once, or (kSpread) to the rows of its choices.  The row
+// is read once: a thread keeps its first kHold packs in registers between the maximum and the rounding, and
+// re-reads the rest.  What a thread does once a row (addresses, the maximum over the group, the scale) costs as
+// much as quantising some five packs, and instructions bound the kernel; so a thread takes four packs, from four
+// threads a row for 128 bfloat16 to 256 for 8,192 (with 256 and two packs for each).  Sixteen packs a thread cost
+// too many registers.
+template <typename T, int N, int L, int kHold, bool kSpread>
 __global__ void __launch_bounds__(kBlock)
     QuantizeRowsKernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int topk,
                        const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
                        int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
     constexpr int kGroups = kBlock / L;
+    using In = Pack<T, N>;
+    using Out = Pack<int8_t, N>;
     __shared__ unsigned int part[kBlock / 32];
     const int group = threadIdx.x / L, at = threadIdx.x % L;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
     const bool real = row < rows;
     const int full = cols / N;
-    const T* xr = x + (real ? row : 0) * ldx;
-    Pack<T, N> hold[kHold];
-    unsigned int top = 0;
     LetLaterStart();
     WaitForEarlier();
+    const T* xr = x + (real ? row : 0) * ldx;
+    const In* packs = reinterpret_cast<const In*>(xr) + at;
+    In hold[kHold];
+    unsigned int top = 0;
     if (real) {
+        // The group's packs of the row, but for its last ones, without a test for each.
+        if (kHold * L <= full) {
 #pragma unroll
-        for (int h = 0; h < kHold; ++h) {
-            const int c = at + h * L;
-            if (c >= full) break;
-            hold[h] = *reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N);
-            top = LargestBits(hold[h], top);
+            for (int h = 0; h < kHold; ++h) hold[h] = packs[h * L];
+        } else {
+#pragma unroll
+            for (int h = 0; h < kHold; ++h) hold[h] = at + h * L < full ? packs[h * L] : In{};
         }
-        for (int c = at + kHold * L; c < full; c += L) {
-            top = LargestBits(*reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N), top);
-        }
-        for (int c = full * N + at; c < cols; c += L) top = max(top, __float_as_uint(ToFloat(xr[c])) & 0x7fffffffu);
+#pragma unroll
+        for (int h = 0; h < kHold; ++h) top = LargestBits(hold[h], top);
+        for (int c = kHold * L; c + at < full; c += L) top = LargestBits(packs[c], top);
+        if (full * N < cols)
+            for (int c = full * N + at; c < cols; c += L) top = max(top, __float_as_uint(ToFloat(xr[c])) & 0x7fffffffu);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (L < 32) {
+        for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    } else {
+        top = __reduce_max_sync(0xffffffffu, top);
+    }
     if constexpr (L > 32) {
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
         __syncthreads();
@@ -154,55 +207,52 @@ __global__ void __launch_bounds__(kBlock)
         for (int w = 0; w < L / 32; ++w) top = max(top, part[group * (L / 32) + w]);
     }
     if (!real) return;
-    const float amax = __uint_as_float(top);
-    const bool finite = top < 0x7f800000u;
-    const bool some = finite && top != 0;
-    const float down = amax > 1e36f ? 0.00390625f : 1.0f;
-    const float inverse = __fdiv_rn(127.0f, amax);
-    const float s = finite ? __fdiv_rn(amax, 127.0f) : __int_as_float(0x7fc00000);
-    const int kept = position ? Kept(offsets, experts, pairs) : 0;
-    const int copies = position ? topk : 1;
-    auto target = [&](int j) -> int64_t {
-        if (!position) return row;
-        const int p = __ldg(position + row * topk + j);
-        return static_cast<unsigned>(p) < static_cast<unsigned>(pairs) ? p : -1;
-    };
-    // Dropped choices get a row of zeros with scale 0.
-    auto store = [&](int c, const Pack<T, N>& v) {
-        Pack<int8_t, N> r{}, zero{};
-        if (some) r = QuantisePack(v, amax, inverse, down);
-        for (int j = 0; j < copies; ++j) {
-            const int64_t to = target(j);
-            if (to >= 0)
-                *reinterpret_cast<Pack<int8_t, N>*>(q + to * ldq + static_cast<int64_t>(c) * N) =
-                    (!position || to < kept) ? r : zero;
+    const RowScale rs = ScaleOf<T>(top);
+    const int kept = kSpread ? Kept(offsets, experts, pairs) : 0;
+    // One row, or one for each choice: zeros (and scale 0) where it was dropped.
+    auto spread = [&](auto&& write) {
+        if constexpr (!kSpread) {
+            write(row, true);
+        } else {
+            for (int j = 0; j < topk; ++j) {
+                const int p = __ldg(position + row * topk + j);
+                if (static_cast<unsigned>(p) < static_cast<unsigned>(pairs)) write(static_cast<int64_t>(p), p < kept);
+            }
         }
     };
+    Out held[kHold];
 #pragma unroll
-    for (int h = 0; h < kHold; ++h) {
-        const int c = at + h * L;
-        if (c >= full) break;
-        store(c, hold[h]);
-    }
-    for (int c = at + kHold * L; c < full; c += L)
-        store(c, *reinterpret_cast<const Pack<T, N>*>(xr + static_cast<int64_t>(c) * N));
-    for (int c = full * N + at; c < cols; c += L) {
-        const int8_t r = some ? static_cast<int8_t>(Quantise(ToFloat(xr[c]), amax, down)) : static_cast<int8_t>(0);
-        for (int j = 0; j < copies; ++j) {
-            const int64_t to = target(j);
-            if (to >= 0) q[to * ldq + c] = (!position || to < kept) ? r : static_cast<int8_t>(0);
+    for (int h = 0; h < kHold; ++h) held[h] = rs.some ? QuantisePack(hold[h], rs) : Out{};
+    spread([&](int64_t to, bool real_row) {
+        Out* qr = reinterpret_cast<Out*>(q + to * ldq) + at;
+        if (real_row && kHold * L <= full) {
+#pragma unroll
+            for (int h = 0; h < kHold; ++h) qr[h * L] = held[h];
+        } else {
+#pragma unroll
+            for (int h = 0; h < kHold; ++h)
+                if (at + h * L < full) qr[h * L] = real_row ? held[h] : Out{};
         }
+    });
+    for (int c = kHold * L; c + at < full; c += L) {
+        const Out r = rs.some ? QuantisePack(packs[c], rs) : Out{};
+        spread([&](int64_t to, bool real_row) { (reinterpret_cast<Out*>(q + to * ldq) + at)[c] = real_row ? r : Out{}; });
     }
-    for (int j = at; j < copies; j += L) {
-        const int64_t to = target(j);
-        if (to >= 0) scale[to] = (!position || to < kept) ? s : 0.0f;
+    if (full * N < cols)
+        for (int c = full * N + at; c < cols; c += L) {
+            const int8_t r = rs.some ? static_cast<int8_t>(Quantise(ToFloat(xr[c]), rs.amax, rs.down)) : static_cast<int8_t>(0);
+            spread([&](int64_t to, bool real_row) { q[to * ldq + c] = real_row ? r : static_cast<int8_t>(0); });
+        }
+    if (at == 0) {
+        const float s = rs.finite ? __fdiv_rn(rs.amax, 127.0f) : __int_as_float(0x7fc00000);
+        spread([&](int64_t to, bool real_row) { scale[to] = real_row ? s : 0.0f; });
     }
 }
 
 // ---- sort by expert ----------------------------------------------------------------------------
 
 // A counting sort over `bins` digits, stable: a tile of keys per block, each of its warps ranking a
-// contiguous piece 32 keys at a time (__match_any_sync gives the lanes that share a digit).  Up to
+// contiguous piece 32 keys at a time (a ballot for each bit of the digit gives the lanes that share it).  Up to
 // kOneBins - 1 experts it is one pass; above that two passes of half the key's bits each, from the low
 // digit to the high one.  A sort that fits one block is one launch; others take three a pass: count, scan
 // each digit over the tiles, scatter.
@@ -221,6 +271,7 @@ struct SortPass {
     const int* keys;   // second pass: the keys and pairs that the first pass left
     const int* pairs;
     int n, experts, shift, mask, bins, tiles;
+    int bits;          // of a digit, `bins` (no key) included
 };
 
 __device__ __forceinline__ int KeyOf(const SortPass& a, int i) {
@@ -231,13 +282,18 @@ __device__ __forceinline__ int KeyOf(const SortPass& a, int i) {
 
 // One round of a warp: each lane's digit (bins: no key) counted into count[]; the lane's rank among the
 // warp's keys of its digit so far.
-__device__ __forceinline__ int CountRound(int d, int bins, unsigned short* count) {
+__device__ __forceinline__ int CountRound(int d, const SortPass& a, unsigned short* count) {
     const int lane = threadIdx.x & 31;
-    const unsigned same = __match_any_sync(0xffffffffu, d);
-    const int before = d < bins ? count[d] : 0;
+    unsigned same = 0xffffffffu;
+    for (int i = 0; i < a.bits; ++i) {
+        const bool set = (d >> i) & 1;
+        const unsigned with = __ballot_sync(0xffffffffu, set);
+        same &= set ? with : ~with;
+    }
+    const int before = d < a.bins ? count[d] : 0;
     const int mine = __popc(same & ((1u << lane) - 1));
     __syncwarp();
-    if (mine == 0 && d < bins) count[d] = static_cast<unsigned short>(before + __popc(same));
+    if (mine == 0 && d < a.bins) count[d] = static_cast<unsigned short>(before + __popc(same));
     __syncwarp();
     return before + mine;
 }
@@ -308,7 +364,7 @@ __global__ void __launch_bounds__(kAloneBlock)
         if (r < rounds) key[r] = first + r * 32 < a.n ? KeyOf(a, first + r * 32) : a.bins;
 #pragma unroll
     for (int r = 0; r < kAloneRounds; ++r)
-        if (r < rounds) rank[r] = static_cast<unsigned short>(CountRound(key[r], a.bins, counts + warp * a.bins));
+        if (r < rounds) rank[r] = static_cast<unsigned short>(CountRound(key[r], a, counts + warp * a.bins));
     __syncthreads();
     ScanDigits(counts, warps, a.bins, base, [](int, int own) { return own; });
     for (int b = threadIdx.x; b < a.bins; b += blockDim.x) offsets[b] = base[b];
@@ -324,64 +380,29 @@ __global__ void __launch_bounds__(kAloneBlock)
 }
 
 // hist[b * tiles + tile] = keys of digit b in the tile.
-__global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* __restrict__ hist, int* __restrict__ totals) {
-    extern __shared__ unsigned short counts[];  // [kSortWarps][bins]
+__global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* __restrict__ hist) {
+    extern __shared__ int base[];  // [bins]
     LetLaterStart();
-    for (int i = threadIdx.x; i < kSortWarps * a.bins; i += kSortBlock) counts[i] = 0;
+    for (int b = threadIdx.x; b < a.bins; b += kSortBlock) base[b] = 0;
     __syncthreads();
     WaitForEarlier();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int first = blockIdx.x * kTile + warp * kPerWarp + lane;
-    int key[kPerWarp / 32];
+    const int first = blockIdx.x * kTile + threadIdx.x;
+    int key[kTile / kSortBlock];
 #pragma unroll
-    for (int r = 0; r < kPerWarp / 32; ++r) key[r] = first + r * 32 < a.n ? KeyOf(a, first + r * 32) : -1;
+    for (int r = 0; r < kTile / kSortBlock; ++r) key[r] = first + r * kSortBlock < a.n ? KeyOf(a, first + r * kSortBlock) : -1;
 #pragma unroll
-    for (int r = 0; r < kPerWarp / 32; ++r) CountRound(key[r] < 0 ? a.bins : (key[r] >> a.shift) & a.mask, a.bins, counts + warp * a.bins);
+    for (int r = 0; r < kTile / kSortBlock; ++r)
+        if (key[r] >= 0) atomicAdd(base + ((key[r] >> a.shift) & a.mask), 1);  // whole numbers: in any order
     __syncthreads();
-    for (int b = threadIdx.x; b < a.bins; b += kSortBlock) {
-        int sum = 0;
-#pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) sum += counts[w * a.bins + b];
-        hist[static_cast<int64_t>(b) * a.tiles + blockIdx.x] = sum;
-    }
-    if (totals)  // two-pass sorts: keys per expert (whole numbers, so the order of the additions is free)
-#pragma unroll
-        for (int r = 0; r < kPerWarp / 32; ++r) {
-            const unsigned same = __match_any_sync(0xffffffffu, key[r]);
-            if (key[r] >= 0 && (same & ((1u << lane) - 1)) == 0) atomicAdd(totals + key[r], __popc(same));
-        }
+    for (int b = threadIdx.x; b < a.bins; b += kSortBlock) hist[static_cast<int64_t>(b) * a.tiles + blockIdx.x] = base[b];
 }
 
-// One warp per digit: its counts to the sums over the tiles before, its total to sums[].  The block after
-// the digits' (two-pass sorts) scans the keys per expert in place.
-constexpr int kScanBlock = 1024;
-__global__ void __launch_bounds__(kScanBlock)
-    SortScanKernel(int* __restrict__ hist, int bins, int tiles, int* __restrict__ sums, int* __restrict__ totals, int experts) {
-    __shared__ int part[32];
+// One warp per digit: its counts to the sums over the tiles before, its total to sums[].
+constexpr int kScanBlock = 256;
+__global__ void __launch_bounds__(kScanBlock) SortScanKernel(int* __restrict__ hist, int bins, int tiles, int* __restrict__ sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     LetLaterStart();
     WaitForEarlier();
-    if (totals && blockIdx.x == gridDim.x - 1) {
-        constexpr int kEach = 8;
-        int carry = 0;
-        for (int e0 = 0; e0 < experts; e0 += kScanBlock * kEach) {
-            const int e = e0 + threadIdx.x * kEach;
-            int v[kEach], own = 0, all;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) v[i] = e + i < experts ? totals[e + i] : 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) own += v[i];
-            int before = carry + ScanThreads(own, part, &all);
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                if (e + i < experts) totals[e + i] = before;
-                before += v[i];
-            }
-            carry += all;
-        }
-        if (threadIdx.x == 0) totals[experts] = carry;  // rows kept: the dropped pairs' count gives way
-        return;
-    }
     const int b = blockIdx.x * (kScanBlock / 32) + warp;
     if (b >= bins) return;
     int* own = hist + static_cast<int64_t>(b) * tiles;
@@ -408,6 +429,21 @@ __global__ void __launch_bounds__(kScanBlock)
     if (lane == 0) sums[b] = carry;
 }
 
+// offsets of a two-pass sort: the first of the sorted keys that is not below e.
+__global__ void SortOffsetsKernel(const int* __restrict__ keys, int n, int experts, int* __restrict__ offsets) {
+    const int e = blockIdx.x * blockDim.x + threadIdx.x;
+    LetLaterStart();
+    WaitForEarlier();
+    if (e > experts) return;
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (__ldg(keys + mid) < e) lo = mid + 1;
+        else hi = mid;
+    }
+    offsets[e] = lo;
+}
+
 // Each key to its place.  offsets (one-pass sorts): where each digit begins.
 __global__ void __launch_bounds__(kSortBlock)
     SortScatterKernel(SortPass a, const int* __restrict__ hist, const int* __restrict__ sums, int* __restrict__ keys_out,
@@ -431,7 +467,7 @@ __global__ void __launch_bounds__(kSortBlock)
 #pragma unroll
     for (int r = 0; r < kPerWarp / 32; ++r)
         rank[r] = static_cast<unsigned short>(
-            CountRound(key[r] < 0 ? a.bins : (key[r] >> a.shift) & a.mask, a.bins, counts + warp * a.bins));
+            CountRound(key[r] < 0 ? a.bins : (key[r] >> a.shift) & a.mask, a, counts + warp * a.bins));
     __syncthreads();
     ScanDigits(counts, kSortWarps, a.bins, base, [&](int b, int) { return sums[b]; });
     if (offsets && blockIdx.x == 0)
@@ -458,7 +494,7 @@ __global__ void ZeroKernel(int* p, int n) {
 
 struct SortPlan {
     int bins[2], shift[2], passes, tiles;
-    size_t sums, keys, pairs, bytes;  // places in the workspace, which begins with the counts of each tile
+    size_t sums, keys, pairs, sorted, bytes;  // places in the workspace, which begins with the counts of each tile
 };
 
 bool Alone(int64_t n, int experts) { return n <= kAlone && experts + 1 <= kOneBins; }
@@ -482,10 +518,11 @@ SortPlan PlanSort(int64_t n, int experts) {
     const size_t most = std::max(p.bins[0], p.bins[1]);
     p.sums = up(most * p.tiles * sizeof(int));
     p.keys = p.sums + up(most * sizeof(int));
-    p.pairs = p.bytes = p.keys;
+    p.pairs = p.sorted = p.bytes = p.keys;
     if (p.passes == 2) {
         p.pairs = p.keys + up(static_cast<size_t>(n) * sizeof(int));
-        p.bytes = p.pairs + up(static_cast<size_t>(n) * sizeof(int));
+        p.sorted = p.pairs + up(static_cast<size_t>(n) * sizeof(int));
+        p.bytes = p.sorted + up(static_cast<size_t>(n) * sizeof(int));
     }
     return p;
 }
@@ -582,24 +619,36 @@ __global__ void __launch_bounds__(kBlock)
         float sum = 0.0f;
         if (p >= 0 && p < kept) {
             const float w = LoadAs(weights, t * topk + j, wtype);
-            for (int c = at; c < full; c += L) {
-                const Pack<T, N> g = *reinterpret_cast<const Pack<T, N>*>(d + static_cast<int64_t>(c) * N);
-                const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(y + p * ldy + static_cast<int64_t>(c) * N);
+            const T* yr = y + p * ldy;
+            T* to = dy + p * lddy;
+            auto one = [&](int c, const Pack<T, N>& g, const Pack<T, N>& v) {
                 Pack<T, N> r;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     sum = fmaf(ToFloat(g.v[i]), ToFloat(v.v[i]), sum);
                     r.v[i] = FromFloat<T>(__fmul_rn(w, ToFloat(g.v[i])));
                 }
-                *reinterpret_cast<Pack<T, N>*>(dy + p * lddy + static_cast<int64_t>(c) * N) = r;
+                *reinterpret_cast<Pack<T, N>*>(to + static_cast<int64_t>(c) * N) = r;
+            };
+            // Two packs of each row in flight; dout's comes from the cache after the first choice.
+            for (int c = at; c < full; c += 2 * L) {
+                const bool two = c + L < full;
+                const int c2 = two ? c + L : c;
+                const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(yr + static_cast<int64_t>(c) * N);
+                const Pack<T, N> v2 = *reinterpret_cast<const Pack<T, N>*>(yr + static_cast<int64_t>(c2) * N);
+                const Pack<T, N> g = *reinterpret_cast<const Pack<T, N>*>(d + static_cast<int64_t>(c) * N);
+                const Pack<T, N> g2 = *reinterpret_cast<const Pack<T, N>*>(d + static_cast<int64_t>(c2) * N);
+                one(c, g, v);
+                if (two) one(c2, g2, v2);
             }
             for (int c = full * N + at; c < cols; c += L) {
                 const float g = ToFloat(d[c]);
-                sum = fmaf(g, ToFloat(y[p * ldy + c]), sum);
-                dy[p * lddy + c] = FromFloat<T>(__fmul_rn(w, g));
+                sum = fmaf(g, ToFloat(yr[c]), sum);
+                to[c] = FromFloat<T>(__fmul_rn(w, g));
             }
         } else if (p >= 0 && p < pairs) {
-            for (int c = at; c < cols; c += L) dy[p * lddy + c] = FromFloat<T>(0.0f);
+            for (int c = at; c < full; c += L) *reinterpret_cast<Pack<T, N>*>(dy + p * lddy + static_cast<int64_t>(c) * N) = Pack<T, N>{};
+            for (int c = full * N + at; c < cols; c += L) dy[p * lddy + c] = FromFloat<T>(0.0f);
         }
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, o);
         if ((threadIdx.x & 31) == 0) part[warp * topk + j] = sum;
@@ -678,18 +727,36 @@ int Quantize(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int6
         constexpr int N = 16 / sizeof(T);
         const T* xp = static_cast<const T*>(x);
         const bool wide = Aligned(x, 16) && ldx % N == 0 && Aligned(q, N) && ldq % N == 0;
-        ForLanes(wide ? cols / N : cols, [&](auto lanes) {
-            constexpr int L = decltype(lanes)::value;
+        const auto launch = [&](auto kernel, int L) {
             const unsigned grid = Blocks(rows, L);
             fits = grid != 0;
-            if (!fits) return;
-            if (wide)
-                error = LaunchAfter(QuantizeRowsKernel<T, N, L>, grid, kBlock, 0, s, xp, ldx, rows, cols, topk, position, offsets, experts,
-                                                                    pairs, q, ldq, scale);
-            else
-                error = LaunchAfter(QuantizeRowsKernel<T, 1, L>, grid, kBlock, 0, s, xp, ldx, rows, cols, topk, position, offsets, experts,
-                                                                    pairs, q, ldq, scale);
-        });
+            if (fits) error = LaunchAfter(kernel, grid, kBlock, 0, s, xp, ldx, rows, cols, topk, position, offsets, experts, pairs, q, ldq, scale);
+        };
+        const auto lay = [&](auto lanes, auto held) {
+            constexpr int L = decltype(lanes)::value, H = decltype(held)::value;
+            if (position) launch(QuantizeRowsKernel<T, N, L, H, true>, L);
+            else launch(QuantizeRowsKernel<T, N, L, H, false>, L);
+        };
+        using std::integral_constant;
+        const int packs = cols / N;
+        if (!wide && cols <= 128) {
+            if (position) launch(QuantizeRowsKernel<T, 1, 32, 4, true>, 32);
+            else launch(QuantizeRowsKernel<T, 1, 32, 4, false>, 32);
+        } else if (!wide) {
+            if (position) launch(QuantizeRowsKernel<T, 1, 256, 4, true>, 256);
+            else launch(QuantizeRowsKernel<T, 1, 256, 4, false>, 256);
+        } else if (packs > 64 && rows < 4 * static_cast<int64_t>(k->num_sms)) {
+            lay(integral_constant<int, 256>{}, integral_constant<int, 2>{});  // few rows: the time of one counts
+        } else {
+            const integral_constant<int, 4> four;
+            if (packs <= 16) lay(integral_constant<int, 4>{}, four);
+            else if (packs <= 32) lay(integral_constant<int, 8>{}, four);
+            else if (packs <= 64) lay(integral_constant<int, 16>{}, four);
+            else if (packs <= 128) lay(integral_constant<int, 32>{}, four);
+            else if (packs <= 256) lay(integral_constant<int, 64>{}, four);
+            else if (packs <= 512) lay(integral_constant<int, 128>{}, four);
+            else lay(integral_constant<int, 256>{}, four);
+        }
     });
     if (!fits) return Bad("too many rows");
     return Ck(error, "quantize_rows");
@@ -745,7 +812,12 @@ int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtyp
         if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (n == 0) return Ck(LaunchAfter(ZeroKernel, std::min(experts / 256 + 1, 64), 256, 0, s, offsets, experts + 1), "sort_by_expert");
-        SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, nullptr, n, experts, 0, 0x7fffffff, experts + 1, p.tiles};
+        const auto bits = [](int bins) {
+            int n_bits = 1;
+            while ((bins >> n_bits) != 0) ++n_bits;
+            return n_bits;
+        };
+        SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, nullptr, n, experts, 0, 0x7fffffff, experts + 1, p.tiles, bits(experts + 1)};
         const size_t most = 72 << 10;
         if (Alone(n, experts)) {
             if (int rc = Ck(cudaFuncSetAttribute(SortAloneKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
@@ -760,21 +832,21 @@ int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtyp
         int* keys = reinterpret_cast<int*>(ws + p.keys);
         int* pairs = reinterpret_cast<int*>(ws + p.pairs);
         if (int rc = Ck(cudaFuncSetAttribute(SortScatterKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
-        if (int rc = Ck(cudaFuncSetAttribute(SortCountKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
-        const auto pass = [&](const SortPass& x, int* totals, int* keys_out, int* pairs_out, int* position_out, int* offsets_out) {
-            const size_t smem = SortSmem(kSortWarps, x.bins);
-            const int digits = (x.bins + kScanBlock / 32 - 1) / (kScanBlock / 32);
-            if (int rc = Ck(LaunchAfter(SortCountKernel, p.tiles, kSortBlock, smem, s, x, hist, totals), "sort_by_expert")) return rc;
-            if (int rc = Ck(LaunchAfter(SortScanKernel, digits + (totals ? 1 : 0), kScanBlock, 0, s, hist, x.bins, p.tiles, sums, totals, experts), "sort_by_expert")) return rc;
-            return Ck(LaunchAfter(SortScatterKernel, p.tiles, kSortBlock, smem, s, x, hist, sums, keys_out, pairs_out, position_out, offsets_out), "sort_by_expert");
+        int* sorted = reinterpret_cast<int*>(ws + p.sorted);
+        const auto pass = [&](const SortPass& x, int* keys_out, int* pairs_out, int* position_out, int* offsets_out) {
+            const int blocks = (x.bins + kScanBlock / 32 - 1) / (kScanBlock / 32);
+            if (int rc = Ck(LaunchAfter(SortCountKernel, p.tiles, kSortBlock, x.bins * sizeof(int), s, x, hist), "sort_by_expert")) return rc;
+            if (int rc = Ck(LaunchAfter(SortScanKernel, blocks, kScanBlock, 0, s, hist, x.bins, p.tiles, sums), "sort_by_expert")) return rc;
+            return Ck(LaunchAfter(SortScatterKernel, p.tiles, kSortBlock, SortSmem(kSortWarps, x.bins), s, x, hist, sums, keys_out, pairs_out, position_out, offsets_out), "sort_by_expert");
         };
-        if (p.passes == 1) return pass(a, nullptr, nullptr, order, position, offsets);
-        if (int rc = Ck(LaunchAfter(ZeroKernel, std::min(experts / 256 + 1, 64), 256, 0, s, offsets, experts + 1), "sort_by_expert")) return rc;
+        if (p.passes == 1) return pass(a, nullptr, order, position, offsets);
         a.mask = p.bins[0] - 1;
         a.bins = p.bins[0];
-        if (int rc = pass(a, offsets, keys, pairs, nullptr, nullptr)) return rc;
-        const SortPass b{nullptr, 0, keys, pairs, n, experts, p.shift[1], 0x7fffffff, p.bins[1], p.tiles};
-        return pass(b, nullptr, nullptr, order, position, nullptr);
+        a.bits = bits(a.bins);
+        if (int rc = pass(a, keys, pairs, nullptr, nullptr)) return rc;
+        const SortPass b{nullptr, 0, keys, pairs, n, experts, p.shift[1], 0x7fffffff, p.bins[1], p.tiles, bits(p.bins[1])};
+        if (int rc = pass(b, sorted, order, position, nullptr)) return rc;
+        return Ck(LaunchAfter(SortOffsetsKernel, experts / 256 + 1, 256, 0, s, sorted, n, experts, offsets), "sort_by_expert");
     });
 }
 
