@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -77,7 +78,7 @@ struct Args {
     const at::Tensor* Maybe(int i, const char* name) const { return v[i] == Py_None ? nullptr : &Tensor(i, name); }
     void* Stream() const { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
     at::Tensor Empty(at::IntArrayRef shape, at::ScalarType type) const {
-        return at::empty(shape, at::TensorOptions().dtype(type).device(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))));
+        return at::detail::empty_cuda(shape, type, c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device)), std::nullopt);
     }
 };
 

@@ -70,7 +70,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
         cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(NVCC))), "include")
         cmd = [HOST_CXX, "-O2", "-std=c++17", "-shared", "-fPIC", BINDING, "-o", BINDING_OUT, "-I", inc, "-I",
                os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_path("include"), "-I", cuda, "-L", lib,
-               "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath," + lib]
+               "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath," + lib]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)

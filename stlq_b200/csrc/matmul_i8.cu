@@ -531,7 +531,7 @@ struct Operands {
     int64_t ldq;
     const int8_t* w;
     int64_t ldw;
-    int sms;
+    int sms, device;
     cudaStream_t stream;
 };
 
@@ -564,7 +564,13 @@ cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
     const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kAllOut + (2 * S::kStages + 4) * 8 + 16 +
                         4 * kWriters * S::kOwnRows + (a.offsets ? (3 * static_cast<size_t>(a.experts) + 1) * 4 : 0);
     const auto kernel = MatmulI8Kernel<kRows, kMode, T>;
-    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); e != cudaSuccess) return e;
+    // Once for each device, as the call takes longer than the rest of the host's work.
+    static thread_local uint64_t set_on = 0;
+    const uint64_t bit = o.device < 64 ? uint64_t{1} << o.device : 0;
+    if (!(set_on & bit)) {
+        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); e != cudaSuccess) return e;
+        set_on |= bit;
+    }
     const int64_t tiles = MostRowTiles(a, kRows) * ((a.n + S::kTileChannels - 1) / S::kTileChannels);
     const int64_t clusters = kMode == kSplit ? tiles : std::min<int64_t>(o.sms / cluster, tiles);
     cudaLaunchConfig_t config{};
@@ -669,7 +675,7 @@ int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_sc
     const int tma_out = Aligned(out, 16) && ldo * out_bytes % 16 == 0 && ldo < (int64_t{1} << 37);
     const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, tma_out, 8, out, ldo,
                        static_cast<unsigned int*>(k->err.p)};
-    const Operands o{q, ldq, w, ldw, k->num_sms, static_cast<cudaStream_t>(stream)};
+    const Operands o{q, ldq, w, ldw, k->num_sms, k->device, static_cast<cudaStream_t>(stream)};
     if (out_dtype == STLQ_B200_F32) return Ck(Launch<float>(o, a), "matmul_i8");
     if (out_dtype == STLQ_B200_BF16) return Ck(Launch<__nv_bfloat16>(o, a), "matmul_i8");
     return Ck(Launch<__half>(o, a), "matmul_i8");

@@ -268,24 +268,24 @@ constexpr int kAlone = kAloneBlock * kAloneRounds;       // the most pairs of a 
 struct SortPass {
     const void* ids;   // first pass: the caller's ids
     int wide;          // ids are int64
-    const int* keys;   // second pass: the keys and pairs that the first pass left
-    const int* pairs;
+    const int2* records;  // second pass: the keys and pairs that the first pass left
     int n, experts, shift, mask, bins, tiles;
-    int bits;          // of a digit, `bins` (no key) included
 };
 
 __device__ __forceinline__ int KeyOf(const SortPass& a, int i) {
-    if (a.keys) return a.keys[i];
+    if (a.records) return a.records[i].x;
     const int64_t id = a.wide ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int*>(a.ids)[i];
     return id >= 0 && id < a.experts ? static_cast<int>(id) : a.experts;
 }
 
-// One round of a warp: each lane's digit (bins: no key) counted into count[]; the lane's rank among the
+// One round of a warp: each lane's digit (bins: no key; below 2^kBits) counted into count[]; the lane's rank among the
 // warp's keys of its digit so far.
+template <int kBits>
 __device__ __forceinline__ int CountRound(int d, const SortPass& a, unsigned short* count) {
     const int lane = threadIdx.x & 31;
     unsigned same = 0xffffffffu;
-    for (int i = 0; i < a.bits; ++i) {
+#pragma unroll
+    for (int i = 0; i < kBits; ++i) {
         const bool set = (d >> i) & 1;
         const unsigned with = __ballot_sync(0xffffffffu, set);
         same &= set ? with : ~with;
@@ -333,6 +333,7 @@ __device__ __forceinline__ void ScanDigits(unsigned short* counts, int warps, in
         const int b = b0 + threadIdx.x;
         int own = 0;
         if (b < bins)
+#pragma unroll 8
             for (int w = 0; w < warps; ++w) {
                 const int c = counts[w * bins + b];
                 counts[w * bins + b] = static_cast<unsigned short>(own);
@@ -347,6 +348,7 @@ __device__ __forceinline__ void ScanDigits(unsigned short* counts, int warps, in
 }
 
 // The whole sort in one block.
+template <int kBits>
 __global__ void __launch_bounds__(kAloneBlock)
     SortAloneKernel(SortPass a, int rounds, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
     extern __shared__ int base[];  // [bins], then the counts [warps][bins]
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(kAloneBlock)
         if (r < rounds) key[r] = first + r * 32 < a.n ? KeyOf(a, first + r * 32) : a.bins;
 #pragma unroll
     for (int r = 0; r < kAloneRounds; ++r)
-        if (r < rounds) rank[r] = static_cast<unsigned short>(CountRound(key[r], a, counts + warp * a.bins));
+        if (r < rounds) rank[r] = static_cast<unsigned short>(CountRound<kBits>(key[r], a, counts + warp * a.bins));
     __syncthreads();
     ScanDigits(counts, warps, a.bins, base, [](int, int own) { return own; });
     for (int b = threadIdx.x; b < a.bins; b += blockDim.x) offsets[b] = base[b];
@@ -429,25 +431,31 @@ __global__ void __launch_bounds__(kScanBlock) SortScanKernel(int* __restrict__ h
     if (lane == 0) sums[b] = carry;
 }
 
-// offsets of a two-pass sort: the first of the sorted keys that is not below e.
-__global__ void SortOffsetsKernel(const int* __restrict__ keys, int n, int experts, int* __restrict__ offsets) {
-    const int e = blockIdx.x * blockDim.x + threadIdx.x;
+// offsets of a two-pass sort: r is the first row of every expert after the key of row r - 1, up to row r's.
+// A warp fills such a stretch together, as it may be as long as there are experts.
+__global__ void SortOffsetsKernel(const int* __restrict__ sorted, int n, int experts, int* __restrict__ offsets) {
     LetLaterStart();
     WaitForEarlier();
-    if (e > experts) return;
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (__ldg(keys + mid) < e) lo = mid + 1;
-        else hi = mid;
+    const int lane = threadIdx.x & 31;
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    int after = 0, to = -1;
+    if (r <= n) {
+        after = r > 0 ? sorted[r - 1] : -1;
+        to = r < n ? sorted[r] : experts;
     }
-    offsets[e] = lo;
+    for (unsigned left = __ballot_sync(0xffffffffu, after < to); left; left &= left - 1) {
+        const int from = __ffs(left) - 1;
+        const int a = __shfl_sync(0xffffffffu, after, from), b = __shfl_sync(0xffffffffu, to, from);
+        for (int e = a + 1 + lane; e <= b; e += 32) offsets[e] = r - lane + from;
+    }
 }
 
-// Each key to its place.  offsets (one-pass sorts): where each digit begins.
+// Each key to its place: the first of two passes writes records, the last one the order, the positions and
+// (two passes) the sorted keys.  offsets (one pass): where each digit begins.
+template <int kBits>
 __global__ void __launch_bounds__(kSortBlock)
-    SortScatterKernel(SortPass a, const int* __restrict__ hist, const int* __restrict__ sums, int* __restrict__ keys_out,
-                      int* __restrict__ pairs_out, int* __restrict__ position, int* __restrict__ offsets) {
+    SortScatterKernel(SortPass a, const int* __restrict__ hist, const int* __restrict__ sums, int2* __restrict__ records,
+                      int* __restrict__ sorted, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
     extern __shared__ int base[];  // [bins], then the counts [kSortWarps][bins]
     unsigned short* counts = reinterpret_cast<unsigned short*>(base + a.bins);
     LetLaterStart();
@@ -461,13 +469,22 @@ __global__ void __launch_bounds__(kSortBlock)
 #pragma unroll
     for (int r = 0; r < kPerWarp / 32; ++r) {
         const int i = first + r * 32;
-        key[r] = i < a.n ? KeyOf(a, i) : -1;
-        pair[r] = i < a.n && a.pairs ? a.pairs[i] : i;
+        key[r] = -1;
+        pair[r] = i;
+        if (i < a.n) {
+            if (a.records) {
+                const int2 v = a.records[i];
+                key[r] = v.x;
+                pair[r] = v.y;
+            } else {
+                key[r] = KeyOf(a, i);
+            }
+        }
     }
 #pragma unroll
     for (int r = 0; r < kPerWarp / 32; ++r)
         rank[r] = static_cast<unsigned short>(
-            CountRound(key[r] < 0 ? a.bins : (key[r] >> a.shift) & a.mask, a, counts + warp * a.bins));
+            CountRound<kBits>(key[r] < 0 ? a.bins : (key[r] >> a.shift) & a.mask, a, counts + warp * a.bins));
     __syncthreads();
     ScanDigits(counts, kSortWarps, a.bins, base, [&](int b, int) { return sums[b]; });
     if (offsets && blockIdx.x == 0)
@@ -480,9 +497,13 @@ __global__ void __launch_bounds__(kSortBlock)
         if (key[r] < 0) continue;
         const int d = (key[r] >> a.shift) & a.mask;
         const int to = base[d] + counts[warp * a.bins + d] + rank[r];
-        pairs_out[to] = pair[r];
-        if (keys_out) keys_out[to] = key[r];
-        if (position) position[pair[r]] = to;
+        if (records) {
+            records[to] = make_int2(key[r], pair[r]);
+        } else {
+            order[to] = pair[r];
+            position[pair[r]] = to;
+            if (sorted) sorted[to] = key[r];
+        }
     }
 }
 
@@ -494,7 +515,7 @@ __global__ void ZeroKernel(int* p, int n) {
 
 struct SortPlan {
     int bins[2], shift[2], passes, tiles;
-    size_t sums, keys, pairs, sorted, bytes;  // places in the workspace, which begins with the counts of each tile
+    size_t sums, records, sorted, bytes;  // places in the workspace, which begins with the counts of each tile
 };
 
 bool Alone(int64_t n, int experts) { return n <= kAlone && experts + 1 <= kOneBins; }
@@ -517,11 +538,10 @@ SortPlan PlanSort(int64_t n, int experts) {
     const auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     const size_t most = std::max(p.bins[0], p.bins[1]);
     p.sums = up(most * p.tiles * sizeof(int));
-    p.keys = p.sums + up(most * sizeof(int));
-    p.pairs = p.sorted = p.bytes = p.keys;
+    p.records = p.sums + up(most * sizeof(int));
+    p.sorted = p.bytes = p.records;
     if (p.passes == 2) {
-        p.pairs = p.keys + up(static_cast<size_t>(n) * sizeof(int));
-        p.sorted = p.pairs + up(static_cast<size_t>(n) * sizeof(int));
+        p.sorted = p.records + up(static_cast<size_t>(n) * sizeof(int2));
         p.bytes = p.sorted + up(static_cast<size_t>(n) * sizeof(int));
     }
     return p;
@@ -571,14 +591,23 @@ __global__ void __launch_bounds__(kBlock)
         float acc[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-        for (int j = 0; j < topk; ++j) {
-            const unsigned p = static_cast<unsigned>(__ldg(position + t * topk + j));
-            if (p >= kept) continue;
-            const float w = weights ? LoadAs(weights, t * topk + j, wtype) : 1.0f;
-            const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(y + p * ldy + static_cast<int64_t>(c) * N);
+        // Four choices' rows in flight; a dropped one adds nothing (its row may hold anything, so it is not a
+        // product with 0).
+        for (int j0 = 0; j0 < topk; j0 += 4) {
+            unsigned p[4];
+            Pack<T, N> v[4];
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = fmaf(w, ToFloat(v.v[i]), acc[i]);
+            for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? static_cast<unsigned>(__ldg(position + t * topk + j0 + j)) : kept;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p[j] < kept) v[j] = *reinterpret_cast<const Pack<T, N>*>(y + p[j] * ldy + static_cast<int64_t>(c) * N);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p[j] < kept) {
+                    const float w = weights ? LoadAs(weights, t * topk + j0 + j, wtype) : 1.0f;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] = fmaf(w, ToFloat(v[j].v[i]), acc[i]);
+                }
         }
         Pack<T, N> r;
 #pragma unroll
@@ -669,6 +698,24 @@ int64_t SizeOf(int dtype) { return dtype == STLQ_B200_F32 ? 4 : 2; }
 bool Aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(to) == 0; }
 int Bad(const char* msg) { return SetError(STLQ_B200_EINVAL, msg); }
 
+// Sets a kernel's dynamic shared memory limit, once for each device.
+template <typename K>
+cudaError_t MostSmem(K kernel, size_t bytes) {
+    struct Seen {
+        const void* kernel;
+        int device;
+    };
+    static thread_local Seen seen[8];
+    static thread_local int used = 0;
+    int device = 0;
+    if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
+    for (int i = 0; i < used; ++i)
+        if (seen[i].kernel == reinterpret_cast<const void*>(kernel) && seen[i].device == device) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess && used < 8) seen[used++] = {reinterpret_cast<const void*>(kernel), device};
+    return e;
+}
+
 template <typename F>
 int Guard(F&& f) {
     try {
@@ -685,11 +732,14 @@ void ForType(int dtype, F&& f) {
     else f(__half{});
 }
 
-// Threads per row: enough that a thread has at most four packs of it, a warp for short rows.
+// Threads per row: a warp for short rows, otherwise enough that a thread has at most four packs of it; more where
+// there are few rows, up to one pack a thread, as the time that one row takes is then the call's.
 template <typename F>
-void ForLanes(int64_t packs, F&& f) {
-    if (packs <= 128) f(std::integral_constant<int, 32>{});
-    else if (packs <= 512) f(std::integral_constant<int, 128>{});
+void ForLanes(int64_t packs, int64_t rows, int sms, F&& f) {
+    int lanes = packs <= 128 ? 32 : packs <= 512 ? 128 : 256;
+    if (rows * lanes < 1024 * static_cast<int64_t>(sms)) lanes = packs <= 32 ? 32 : packs <= 128 ? 128 : 256;
+    if (lanes == 32) f(std::integral_constant<int, 32>{});
+    else if (lanes == 128) f(std::integral_constant<int, 128>{});
     else f(std::integral_constant<int, 256>{});
 }
 
@@ -745,8 +795,10 @@ int Quantize(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int6
         } else if (!wide) {
             if (position) launch(QuantizeRowsKernel<T, 1, 256, 4, true>, 256);
             else launch(QuantizeRowsKernel<T, 1, 256, 4, false>, 256);
-        } else if (packs > 64 && rows < 4 * static_cast<int64_t>(k->num_sms)) {
-            lay(integral_constant<int, 256>{}, integral_constant<int, 2>{});  // few rows: the time of one counts
+        } else if (packs > 32 && rows * ((packs + 3) / 4) < 1024 * static_cast<int64_t>(k->num_sms)) {
+            // Few rows: the time of one counts.
+            if (packs <= 128) lay(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+            else lay(integral_constant<int, 256>{}, integral_constant<int, 2>{});
         } else {
             const integral_constant<int, 4> four;
             if (packs <= 16) lay(integral_constant<int, 4>{}, four);
@@ -812,41 +864,36 @@ int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtyp
         if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (n == 0) return Ck(LaunchAfter(ZeroKernel, std::min(experts / 256 + 1, 64), 256, 0, s, offsets, experts + 1), "sort_by_expert");
-        const auto bits = [](int bins) {
-            int n_bits = 1;
-            while ((bins >> n_bits) != 0) ++n_bits;
-            return n_bits;
-        };
-        SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, nullptr, n, experts, 0, 0x7fffffff, experts + 1, p.tiles, bits(experts + 1)};
+        SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, n, experts, 0, 0x7fffffff, experts + 1, p.tiles};
         const size_t most = 72 << 10;
         if (Alone(n, experts)) {
-            if (int rc = Ck(cudaFuncSetAttribute(SortAloneKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
             // As many warps as there are rounds for, so that few pairs take one round.
             const int warps = std::min(kAloneBlock / 32, (n + 31) / 32);
             const int rounds = (n + warps * 32 - 1) / (warps * 32);
-            return Ck(LaunchAfter(SortAloneKernel, 1, warps * 32, SortSmem(warps, a.bins), s, a, rounds, order, position, offsets), "sort_by_expert");
+            const auto kernel = a.bins < 256 ? SortAloneKernel<8> : SortAloneKernel<11>;
+            if (int rc = Ck(MostSmem(kernel, most), "sort_by_expert")) return rc;
+            return Ck(LaunchAfter(kernel, 1, warps * 32, SortSmem(warps, a.bins), s, a, rounds, order, position, offsets), "sort_by_expert");
         }
         char* ws = static_cast<char*>(workspace);
         int* hist = reinterpret_cast<int*>(ws);
         int* sums = reinterpret_cast<int*>(ws + p.sums);
-        int* keys = reinterpret_cast<int*>(ws + p.keys);
-        int* pairs = reinterpret_cast<int*>(ws + p.pairs);
-        if (int rc = Ck(cudaFuncSetAttribute(SortScatterKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most), "sort_by_expert")) return rc;
+        int2* records = reinterpret_cast<int2*>(ws + p.records);
         int* sorted = reinterpret_cast<int*>(ws + p.sorted);
-        const auto pass = [&](const SortPass& x, int* keys_out, int* pairs_out, int* position_out, int* offsets_out) {
+        const auto pass = [&](const SortPass& x, int2* records_out, int* sorted_out, int* offsets_out) {
             const int blocks = (x.bins + kScanBlock / 32 - 1) / (kScanBlock / 32);
+            const auto scatter = x.bins < 256 ? SortScatterKernel<8> : SortScatterKernel<11>;
+            if (int rc = Ck(MostSmem(scatter, most), "sort_by_expert")) return rc;
             if (int rc = Ck(LaunchAfter(SortCountKernel, p.tiles, kSortBlock, x.bins * sizeof(int), s, x, hist), "sort_by_expert")) return rc;
             if (int rc = Ck(LaunchAfter(SortScanKernel, blocks, kScanBlock, 0, s, hist, x.bins, p.tiles, sums), "sort_by_expert")) return rc;
-            return Ck(LaunchAfter(SortScatterKernel, p.tiles, kSortBlock, SortSmem(kSortWarps, x.bins), s, x, hist, sums, keys_out, pairs_out, position_out, offsets_out), "sort_by_expert");
+            return Ck(LaunchAfter(scatter, p.tiles, kSortBlock, SortSmem(kSortWarps, x.bins), s, x, hist, sums, records_out, sorted_out, order, position, offsets_out), "sort_by_expert");
         };
-        if (p.passes == 1) return pass(a, nullptr, order, position, offsets);
+        if (p.passes == 1) return pass(a, nullptr, nullptr, offsets);
         a.mask = p.bins[0] - 1;
         a.bins = p.bins[0];
-        a.bits = bits(a.bins);
-        if (int rc = pass(a, keys, pairs, nullptr, nullptr)) return rc;
-        const SortPass b{nullptr, 0, keys, pairs, n, experts, p.shift[1], 0x7fffffff, p.bins[1], p.tiles, bits(p.bins[1])};
-        if (int rc = pass(b, sorted, order, position, nullptr)) return rc;
-        return Ck(LaunchAfter(SortOffsetsKernel, experts / 256 + 1, 256, 0, s, sorted, n, experts, offsets), "sort_by_expert");
+        if (int rc = pass(a, records, nullptr, nullptr)) return rc;
+        const SortPass b{nullptr, 0, records, n, experts, p.shift[1], 0x7fffffff, p.bins[1], p.tiles};
+        if (int rc = pass(b, nullptr, sorted, nullptr)) return rc;
+        return Ck(LaunchAfter(SortOffsetsKernel, n / 256 + 1, 256, 0, s, sorted, n, experts, offsets), "sort_by_expert");
     });
 }
 
@@ -872,7 +919,7 @@ int stlq_b200_dispatch(stlq_b200_kernels* k, const void* x, int elem_bytes, int6
         auto launch = [&](auto pack) {
             using V = decltype(pack);
             const int packs = bytes / static_cast<int>(sizeof(V));
-            ForLanes(packs, [&](auto lanes) {
+            ForLanes(packs, tokens, k->num_sms, [&](auto lanes) {
                 constexpr int L = decltype(lanes)::value;
                 const unsigned grid = Blocks(tokens, L);
                 fits = grid != 0;
@@ -916,7 +963,7 @@ int stlq_b200_combine(stlq_b200_kernels* k, const void* y, int dtype, int64_t ld
             using T = decltype(one);
             constexpr int N = 16 / sizeof(T);
             const bool wide = Aligned(y, 16) && ldy % N == 0 && Aligned(out, 16) && ldo % N == 0;
-            ForLanes(wide ? cols / N : cols, [&](auto lanes) {
+            ForLanes(wide ? cols / N : cols, tokens, k->num_sms, [&](auto lanes) {
                 constexpr int L = decltype(lanes)::value;
                 const unsigned grid = Blocks(tokens, L);
                 fits = grid != 0;
@@ -961,7 +1008,7 @@ int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype
             using T = decltype(one);
             constexpr int N = 16 / sizeof(T);
             const bool wide = Aligned(dout, 16) && ldd % N == 0 && Aligned(y, 16) && ldy % N == 0 && Aligned(dy, 16) && lddy % N == 0;
-            ForLanes(wide ? cols / N : cols, [&](auto lanes) {
+            ForLanes(wide ? cols / N : cols, tokens, k->num_sms, [&](auto lanes) {
                 constexpr int L = decltype(lanes)::value;
                 const unsigned grid = Blocks(tokens, L);
                 fits = grid != 0;
