@@ -47,20 +47,20 @@ struct alignas(sizeof(T) * N) Pack {
     T v[N];
 };
 
-// Accesses whose lines leave the cache first, for what is read or written once and is larger than it
-// (combine of 16,384 x 8 x 2,048 bfloat16: 99 us without, 93 with; its gradient 200 and 191).
+// Accesses whose lines leave the cache first, for what is read or written once and is larger than it: combine's
+// y (16,384 x 8 x 2,048 bfloat16: 98 us without, 92 with) and its gradient's dy (199 and 191).  The gradient's y is
+// read the ordinary way (184; 187 otherwise).
 template <typename P>
 __device__ __forceinline__ void StoreStreaming(void* to, const P& v) {
     if constexpr (sizeof(P) == 16) __stcs(static_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&v));
     else *static_cast<P*>(to) = v;
 }
 
-template <typename P>
-__device__ __forceinline__ P LoadStreaming(const void* from) {
-    P v;
-    if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4*>(&v) = __ldcs(static_cast<const uint4*>(from));
+template <bool kStreaming, typename P>
+__device__ __forceinline__ void Load(P& v, const void* from) {
+    if constexpr (sizeof(P) == 16 && kStreaming) *reinterpret_cast<uint4*>(&v) = __ldcs(static_cast<const uint4*>(from));
+    else if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4*>(&v) = *static_cast<const uint4*>(from);
     else v = *static_cast<const P*>(from);
-    return v;
 }
 
 __device__ __forceinline__ float LoadAs(const void* p, int64_t i, int dtype) {
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kBlock)
             for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? static_cast<unsigned>(__ldg(position + t * topk + j0 + j)) : kept;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (p[j] < kept) v[j] = LoadStreaming<Pack<T, N>>(y + p[j] * ldy + static_cast<int64_t>(c) * N);
+                if (p[j] < kept) Load<true>(v[j], y + p[j] * ldy + static_cast<int64_t>(c) * N);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (p[j] < kept) {
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(kBlock, 4)
             Pack<T, N> v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (p[j] >= 0 && p[j] < kept) v[j] = LoadStreaming<Pack<T, N>>(y + p[j] * ldy + e);
+                if (p[j] >= 0 && p[j] < kept) Load<false>(v[j], y + p[j] * ldy + e);
             const Pack<T, N> g = real ? *reinterpret_cast<const Pack<T, N>*>(d + e) : Pack<T, N>{};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
