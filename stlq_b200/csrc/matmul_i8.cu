@@ -46,14 +46,15 @@ template <int kRows, Mode kMode, typename T>
 struct Shape {
     static constexpr uint32_t kXBytes = (kMode == kPair ? kRows / 2 : kRows) * kTileK;
     static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
-    // Where a writing warp lays out 16 rows of its 32 channels for a TMA store, twice.
-    static constexpr uint32_t kOutBytes = 16 * 32 * sizeof(T);
+    // A writing warp takes this many rows of its 32 channels at a time, and lays them out for a TMA store, twice.
+    static constexpr int kChunk = kMode != kSplit && kRows >= 128 ? 32 : 16;
+    static constexpr uint32_t kOutBytes = kChunk * 32 * sizeof(T);
     static constexpr uint32_t kAllOut = kMode == kSplit ? 0 : 2 * kWriters * kOutBytes;
     static constexpr int kStages = std::min<int>(10, (209 * 1024 - kAllOut) / kStageBytes);
     static constexpr int kColumns = kRows < 32 ? 32 : kRows;        // TMEM columns of one accumulator
     static constexpr uint32_t kTmem = (kMode == kSplit ? 1 : 2) * kColumns;  // two: one is written out while the next is made
     static constexpr int kTileChannels = kMode == kPair ? 2 * kChannels : kChannels;
-    static constexpr int kOwnRows = std::max(16, kRows / kShare);   // rows of the tile that a writing warp takes
+    static constexpr int kOwnRows = std::max(kChunk, kRows / kShare);   // rows of the tile that a writing warp takes
     static constexpr int kGranule = kMode == kPair ? 32 : 16;       // rows of an MMA come in multiples of this
 };
 
@@ -64,6 +65,7 @@ struct MatmulArgs {
     const int* offsets;  // null: one matrix, all rows
     int experts, rows, n, kdim;
     int tma_out;         // the output's rows begin on 16-byte boundaries
+    int evict_first;     // the output is larger than the L2 cache's share for it
     int band;            // row tiles that run side by side over the channels
     void* out;
     int64_t ldo;
@@ -112,8 +114,7 @@ __device__ __forceinline__ Tile FindTile(const MatmulArgs& a, const Segments& sg
         t.row0 = 0;
         t.end = a.rows;
     }
-    // Bands of row tiles, the band's row tiles running fastest: the tiles in flight share few rows and
-    // few channels, which stay in L2.
+    // Bands of row tiles, the band's row tiles running fastest.
     const int rt = (t.end - t.row0 + kRows - 1) / kRows;
     const int band = local / (a.band * ct), in = local - band * a.band * ct;
     const int height = min(a.band, rt - band * a.band);
@@ -309,8 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp >= 2) {
         const int quarter = warp & 3;  // the TMEM lanes this warp may read
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        // Of every 16 * kShare rows, this warp takes 16.
-        constexpr int kStep = 16 * kShare;
+        // Of every kChunk * kShare rows, this warp takes kChunk.
+        constexpr int kChunk = S::kChunk, kStep = kChunk * kShare;
         const int share = (warp - 2) >> 2;
         float* scales = row_scales + (warp - 2) * S::kOwnRows;
         int* parts = reinterpret_cast<int*>(base);  // kSplit: [kRows][kChannels] over the stages, once they are read
@@ -318,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int done = 0, slot = 0;
         bool ok = true;
         const bool one = tc::ElectOne();
+        const uint64_t policy = tc::CachePolicy(a.evict_first);
         // What a tile needs beside its sums.  The next tile's is on its way while this one is written:
         // with few steps of kdim a tile would otherwise wait for it every time.
         constexpr int kOwn = (S::kOwnRows + 31) / 32;
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int count = min(kRows, x.t.end - x.t.row0);
 #pragma unroll
             for (int i = 0; i < kOwn; ++i) {
-                const int r = i * 32 + lane, row = (r >> 4) * kStep + share * 16 + (r & 15);
+                const int r = i * 32 + lane, row = r / kChunk * kStep + share * kChunk + r % kChunk;
                 x.qs[i] = r < S::kOwnRows && row < count ? a.q_scale[x.t.row0 + row] : 0.0f;
             }
             return x;
@@ -355,68 +357,68 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < kOwn; ++i)
                 if (i * 32 + lane < S::kOwnRows) scales[i * 32 + lane] = now.qs[i];
             __syncwarp();
-            T* direct = out + (static_cast<int64_t>(t.row0) + share * 16) * a.ldo + c;
+            T* direct = out + (static_cast<int64_t>(t.row0) + share * kChunk) * a.ldo + c;
             ok = __all_sync(0xffffffffu, tc::MbarWait(&made[b], (done >> 1) & 1, a.err, kWaitNs));
             if (ok) {
                 tc::FenceAfterSync();
                 const uint32_t from = tmem + lanes + b * S::kColumns;
-                auto write = [&](const int (&v)[16], int c0) {
+                auto write = [&](const int (&v)[kChunk], int c0) {
                     if constexpr (kMode == kSplit) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) parts[(c0 + j) * kChannels + quarter * 32 + lane] = v[j];
+                        for (int j = 0; j < kChunk; ++j) parts[(c0 + j) * kChannels + quarter * 32 + lane] = v[j];
                     } else {
-                        float y[16];
-                        const float4* own = reinterpret_cast<const float4*>(scales + c0 / kShare / 16 * 16);
+                        float y[kChunk];
+                        const float4* own = reinterpret_cast<const float4*>(scales + c0 / kStep * kChunk);
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
+                        for (int j = 0; j < kChunk; j += 4) {
                             const float4 sc = own[j / 4];
                             y[j] = fmaf(__int2float_rn(v[j]) * sc.x, ws, bias);
                             y[j + 1] = fmaf(__int2float_rn(v[j + 1]) * sc.y, ws, bias);
                             y[j + 2] = fmaf(__int2float_rn(v[j + 2]) * sc.z, ws, bias);
                             y[j + 3] = fmaf(__int2float_rn(v[j + 3]) * sc.w, ws, bias);
                         }
-                        // 16 rows of this segment at once by TMA, which also leaves out what is past the
+                        // A chunk of this segment at once by TMA, which also leaves out what is past the
                         // output's edges; rows that belong to the next segment are left out here.
-                        if (a.tma_out && (c0 + 16 <= count || !a.offsets)) {
+                        if (a.tma_out && (c0 + kChunk <= count || !a.offsets)) {
                             T* lay = reinterpret_cast<T*>(outs + (2 * (warp - 2) + slot) * S::kOutBytes);
                             if (one) tc::BulkWaitRead<1>();
                             __syncwarp();
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) lay[j * 32 + lane] = Out<T>(y[j]);
+                            for (int j = 0; j < kChunk; ++j) lay[j * 32 + lane] = Out<T>(y[j]);
                             tc::FenceAsyncShared();
                             __syncwarp();
                             if (one) {
-                                tc::TmaStore2d(&to, lay, c - lane, t.row0 + c0);
+                                tc::TmaStore2d(&to, lay, c - lane, t.row0 + c0, policy);
                                 tc::BulkCommit();
                             }
                             slot ^= 1;
                         } else {
                             const int left = real ? count - c0 : 0;
                             T* row = direct;
-                            if (left >= 16) {
+                            if (left >= kChunk) {
 #pragma unroll
-                                for (int j = 0; j < 16; ++j, row += a.ldo) *row = Out<T>(y[j]);
+                                for (int j = 0; j < kChunk; ++j, row += a.ldo) *row = Out<T>(y[j]);
                             } else {
 #pragma unroll
-                                for (int j = 0; j < 16; ++j, row += a.ldo)
+                                for (int j = 0; j < kChunk; ++j, row += a.ldo)
                                     if (j < left) *row = Out<T>(y[j]);
                             }
                         }
                         direct += kStep * a.ldo;
                     }
                 };
-                // The next 16 columns are on their way while 16 are written.
-                int va[16], vb[16];
-                int c0 = share * 16;
-                if (c0 < count) tc::TmemLoad16(from + c0, va);
+                // The next columns are on their way while these are written.
+                int va[kChunk], vb[kChunk];
+                int c0 = share * kChunk;
+                if (c0 < count) tc::TmemLoad(from + c0, va);
 #pragma unroll 1
                 for (; c0 < count; c0 += 2 * kStep) {
                     tc::TmemLoadWait(va);
-                    if (c0 + kStep < count) tc::TmemLoad16(from + c0 + kStep, vb);
+                    if (c0 + kStep < count) tc::TmemLoad(from + c0 + kStep, vb);
                     write(va, c0);
                     if (c0 + kStep >= count) break;
                     tc::TmemLoadWait(vb);
-                    if (c0 + 2 * kStep < count) tc::TmemLoad16(from + c0 + 2 * kStep, va);
+                    if (c0 + 2 * kStep < count) tc::TmemLoad(from + c0 + 2 * kStep, va);
                     write(vb, c0 + kStep);
                 }
                 tc::FenceBeforeSync();
@@ -559,7 +561,7 @@ cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
                               : std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (kMode != kSplit && a.tma_out &&
-        !MakeMap(&to, kOutType, a.out, a.rows, a.n, a.ldo * static_cast<int64_t>(sizeof(T)), 16, 32))
+        !MakeMap(&to, kOutType, a.out, a.rows, a.n, a.ldo * static_cast<int64_t>(sizeof(T)), S::kChunk, 32))
         return cudaErrorInvalidValue;
     const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kAllOut + (2 * S::kStages + 4) * 8 + 16 +
                         4 * kWriters * S::kOwnRows + (a.offsets ? (3 * static_cast<size_t>(a.experts) + 1) * 4 : 0);
@@ -673,7 +675,13 @@ int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_sc
     const int64_t out_bytes = out_dtype == STLQ_B200_F32 ? 4 : 2;
     // TMA's rows: on 16-byte boundaries, less than 2^40 bytes apart.
     const int tma_out = Aligned(out, 16) && ldo * out_bytes % 16 == 0 && ldo < (int64_t{1} << 37);
-    const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, tma_out, 8, out, ldo,
+    // A large output is written in rows as long as possible, and leaves the cache in that order: tiles run along
+    // the channels and its lines are marked to go first (4,096 x 65,536 x 128 to 32 bits: 220 us without the two,
+    // 205 with the mark, 166 with both, 6.5 TB/s).  A matrix that does not stay in the cache from one row of
+    // tiles to the next is read for eight at a time instead.
+    const int evict_first = static_cast<int64_t>(rows) * n * out_bytes > (int64_t{48} << 20);
+    const int band = static_cast<int64_t>(n) * kdim <= (int64_t{32} << 20) ? 1 : 8;
+    const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, tma_out, evict_first, band, out, ldo,
                        static_cast<unsigned int*>(k->err.p)};
     const Operands o{q, ldq, w, ldw, k->num_sms, k->device, static_cast<cudaStream_t>(stream)};
     if (out_dtype == STLQ_B200_F32) return Ck(Launch<float>(o, a), "matmul_i8");
