@@ -386,7 +386,7 @@ int stlq_b200_matmul_i8_grouped(stlq_b200_kernels* k, const int8_t* q, int64_t l
 /* The pairs p = t * topk + j of ids (tokens x topk, contiguous, STLQ_B200_I32 or _I64) sorted by expert, in the order of
  * p within an expert: order[r] = the pair at sorted row r, position[p] = the sorted row of pair p, offsets[e] = the first
  * row of expert e (experts + 1 values; offsets[experts] = rows kept).  An id outside [0, experts) is a dropped choice:
- * its pair comes after all kept ones.  tokens * topk below 2^31.  workspace: 16-byte aligned, of the bytes that
+ * its pair comes after all kept ones.  tokens * topk at most 2^31 - 1024.  workspace: 16-byte aligned, of the bytes that
  * stlq_b200_sort_by_expert_workspace gives; free again once the call's work is done. */
 int stlq_b200_sort_by_expert_workspace(int64_t tokens, int topk, int experts, size_t* bytes);
 int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtype, int64_t tokens, int topk, int experts,

@@ -400,6 +400,26 @@ PyObject* CombineBackward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// (order, position, offsets) -> tokens, topk, experts
+PyObject* CheckRouting(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return Guard([&]() -> PyObject* {
+        if (n != 3) throw Refused("order, position and offsets are needed");
+        for (int i = 0; i < 3; ++i)
+            if (!THPVariable_Check(args[i])) throw Refused("order, position and offsets must be tensors");
+        const at::Tensor &o = THPVariable_Unpack(args[0]), &p = THPVariable_Unpack(args[1]), &f = THPVariable_Unpack(args[2]);
+        if (o.dim() != 1 || p.dim() != 2 || f.dim() != 1) throw Refused("order, position and offsets must have 1, 2 and 1 dimensions");
+        for (const at::Tensor* t : {&o, &p, &f})
+            if (t->scalar_type() != at::kInt || !t->is_contiguous()) throw Refused("order, position and offsets must be contiguous int32");
+        const int64_t tokens = p.size(0), topk = p.size(1), experts = f.size(0) - 1;
+        if (o.size(0) != tokens * topk) throw Refused("order must have tokens * topk = " + std::to_string(tokens * topk) + " elements");
+        if (topk < 1 || topk > STLQ_B200_MAX_TOPK) throw Refused("topk must be in [1, 64], got " + std::to_string(topk));
+        if (experts < 1 || experts > STLQ_B200_MAX_ROOT) throw Refused("experts must be in [1, 65536], got " + std::to_string(experts));
+        PyObject* t = Py_BuildValue("LLL", static_cast<long long>(tokens), static_cast<long long>(topk), static_cast<long long>(experts));
+        if (!t) throw Raised{};
+        return t;
+    });
+}
+
 // (StlqB200Error, addresses of the entry points in Api's order)
 PyObject* Give(PyObject*, PyObject* const* args, Py_ssize_t n) {
     constexpr Py_ssize_t kCount = sizeof(Api) / sizeof(void*);
@@ -422,6 +442,7 @@ PyObject* Give(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define STLQ_METHOD(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {STLQ_METHOD("give", Give),
+                         STLQ_METHOD("check_routing", CheckRouting),
                          STLQ_METHOD("quantize_rows", QuantizeRows),
                          STLQ_METHOD("matmul_i8", Matmul),
                          STLQ_METHOD("matmul_i8_grouped", MatmulGrouped),

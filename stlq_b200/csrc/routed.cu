@@ -27,6 +27,7 @@ using stlq_b200::SetError;
 using stlq_b200::WaitForEarlier;
 
 constexpr int kBlock = 256;
+constexpr int64_t kMostPairs = 0x7ffffc00;  // so that a block's worth past the last pair is still an int
 
 template <typename T>
 __device__ __forceinline__ float ToFloat(T v) {
@@ -801,7 +802,7 @@ unsigned Blocks(int64_t rows, int L) {
 int CheckRouting(int64_t tokens, int topk, int experts, const void* position, const void* offsets) {
     if (tokens < 0 || topk < 1 || topk > STLQ_B200_MAX_TOPK) return Bad("tokens >= 0 and 1 <= topk <= 64 required");
     if (experts < 1 || experts > STLQ_B200_MAX_ROOT) return Bad("1 <= experts <= 65536 required");
-    if (tokens > 0x7fffffff / topk) return Bad("tokens * topk must be below 2^31");
+    if (tokens > kMostPairs / topk) return Bad("tokens * topk must be at most 2^31 - 1024");
     if (tokens > 0 && (!position || !offsets)) return Bad("null position or offsets");
     if (!Aligned(position, 4) || !Aligned(offsets, 4)) return Bad("position and offsets must be 4-byte aligned");
     return 0;

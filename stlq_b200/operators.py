@@ -19,11 +19,8 @@ elements of a row may not.  Wrong shapes, types, layouts or devices raise ValueE
 from __future__ import annotations
 
 import ctypes
-import os
 
 from .encoder import StlqB200Error, load_library
-
-MAX_TOPK, MAX_SORT_EXPERTS = 64, 65536
 
 _READY = None
 
@@ -60,20 +57,8 @@ class Routing:
     __slots__ = ("order", "position", "offsets", "tokens", "topk", "experts")
 
     def __init__(self, order, position, offsets):
-        if position.dim() != 2 or offsets.dim() != 1 or order.dim() != 1:
-            raise ValueError("order, position and offsets must have 1, 2 and 1 dimensions")
+        self.tokens, self.topk, self.experts = _ready()[1].check_routing(order, position, offsets)
         self.order, self.position, self.offsets = order, position, offsets
-        self.tokens, self.topk = position.shape
-        self.experts = offsets.shape[0] - 1
-        if order.shape[0] != self.tokens * self.topk:
-            raise ValueError(f"order must have tokens * topk = {self.tokens * self.topk} elements, got {order.shape[0]}")
-        if not 1 <= self.topk <= MAX_TOPK:
-            raise ValueError(f"topk must be in [1, {MAX_TOPK}], got {self.topk}")
-        if not 1 <= self.experts <= MAX_SORT_EXPERTS:
-            raise ValueError(f"experts must be in [1, {MAX_SORT_EXPERTS}], got {self.experts}")
-        for t in (order, position, offsets):
-            if str(t.dtype) != "torch.int32" or not t.is_contiguous():
-                raise ValueError("order, position and offsets must be contiguous int32")
 
     def __repr__(self):
         return f"Routing(tokens={self.tokens}, topk={self.topk}, experts={self.experts})"

@@ -164,7 +164,8 @@ def check_product(y, q, s, w, ws, bias, dtype):
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("rows,n,kdim", [(1, 1, 1), (1, 130, 17), (2, 128, 128), (5, 300, 96), (16, 129, 960), (17, 64, 129), (31, 257, 256),
                                          (33, 40, 1000), (64, 128, 4096), (65, 500, 33), (127, 128, 640), (129, 1000, 300), (255, 130, 128),
-                                         (256, 256, 512), (257, 129, 130), (700, 385, 1100), (1, 4096, 4096), (3, 1000, 5000), (1300, 2100, 257)])
+                                         (256, 256, 512), (257, 129, 130), (700, 385, 1100), (1, 4096, 4096), (3, 1000, 5000), (1300, 2100, 257),
+                                         (300, 8, 64), (20, 16, 128), (130, 24, 40), (2000, 32, 70), (100, 136, 8000), (5, 64, 2000), (1100, 4096, 96), (4000, 3000, 260)])
 def test_matmul_i8(k, dtype, rows, n, kdim):
     g = rng_for(3, rows, n, kdim)
     q, w = randq(g, rows, kdim), randq(g, n, kdim)
