@@ -571,3 +571,20 @@ def test_c_entries_refuse(k):
     assert refused == [1] * len(refused)
     assert lib.stlq_b200_last_error()
     k.sync()
+
+
+def test_example_routed_roots():
+    """The example that runs the operators together.  An 8-bit row has at most 1/254 of its largest value's error in each element and
+    so has the matrix; over 128 elements with a largest value some 2 to 4 times their root mean square, each gives about 1 %."""
+    if not have_cuda():
+        pytest.skip("no CUDA device")
+    import importlib.util
+    import os
+
+    from conftest import ROOT
+
+    spec = importlib.util.spec_from_file_location("routed_roots", os.path.join(ROOT, "examples", "routed_roots.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    error, before, after = m.main(vectors=3000, roots=20, dim=128, out_dim=48)
+    assert error < 0.02 and after < before
