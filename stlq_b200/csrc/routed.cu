@@ -279,8 +279,10 @@ __global__ void __launch_bounds__(kBlock)
 // each digit over the tiles, scatter.
 constexpr int kSortBlock = 512;
 constexpr int kSortWarps = kSortBlock / 32;
-constexpr int kPerWarp = 256;
-constexpr int kTile = kSortWarps * kPerWarp;
+// Keys of a warp: more make longer runs of a digit to write, fewer use more SMs (32,768 pairs over 64 experts took
+// 11 us in 8 tiles of the longer ones).
+constexpr int kFewPerWarp = 64, kManyPerWarp = 256;
+constexpr int64_t kFewPairs = 148 * kSortWarps * 2 * kFewPerWarp;
 constexpr int kOneBins = 1025;
 constexpr int kAloneBlock = 1024;
 constexpr int kAloneRounds = 16;                         // keys of a lane
@@ -401,7 +403,9 @@ __global__ void __launch_bounds__(kAloneBlock)
 }
 
 // hist[b * tiles + tile] = keys of digit b in the tile.
+template <int kPerWarp>
 __global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* __restrict__ hist) {
+    constexpr int kTile = kSortWarps * kPerWarp;
     extern __shared__ int base[];  // [bins]
     LetLaterStart();
     for (int b = threadIdx.x; b < a.bins; b += kSortBlock) base[b] = 0;
@@ -473,10 +477,11 @@ __global__ void SortOffsetsKernel(const int* __restrict__ sorted, int n, int exp
 // (two passes) the sorted keys.  offsets (one pass): where each digit begins.  The tile is put in order in shared
 // memory first, so that neighbouring threads write neighbouring elements of a digit (written from where the keys
 // lay, a pass of a million took 27 us, most of them for partly filled sectors).
-template <int kBits>
+template <int kBits, int kPerWarp>
 __global__ void __launch_bounds__(kSortBlock)
     SortScatterKernel(SortPass a, const int* __restrict__ hist, const int* __restrict__ sums, int2* __restrict__ records,
                       int* __restrict__ sorted, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
+    constexpr int kTile = kSortWarps * kPerWarp;
     extern __shared__ int2 tile[];  // [kTile], then the digits' places [2][bins] and the counts [kSortWarps][bins]
     __shared__ int part[32];
     int* local = reinterpret_cast<int*>(tile + kTile);  // of the digit's first key in the tile
@@ -552,7 +557,7 @@ __global__ void ZeroKernel(int* p, int n) {
 }
 
 struct SortPlan {
-    int bins[2], shift[2], passes, tiles;
+    int bins[2], shift[2], passes, tile, tiles;
     size_t sums, records, sorted, bytes;  // places in the workspace, which begins with the counts of each tile
 };
 
@@ -561,7 +566,8 @@ bool Alone(int64_t n, int experts) { return n <= kAlone && experts + 1 <= kOneBi
 SortPlan PlanSort(int64_t n, int experts) {
     SortPlan p{};
     if (Alone(n, experts)) return p;
-    p.tiles = static_cast<int>((n + kTile - 1) / kTile);
+    p.tile = kSortWarps * (n <= kFewPairs ? kFewPerWarp : kManyPerWarp);
+    p.tiles = static_cast<int>((n + p.tile - 1) / p.tile);
     if (experts + 1 <= kOneBins) {
         p.passes = 1;
         p.bins[0] = experts + 1;
@@ -932,11 +938,14 @@ int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtyp
         int* sorted = reinterpret_cast<int*>(ws + p.sorted);
         const auto pass = [&](const SortPass& x, int2* records_out, int* sorted_out, int* offsets_out) {
             const int blocks = (x.bins + kScanBlock / 32 - 1) / (kScanBlock / 32);
-            const auto scatter = x.bins < 256 ? SortScatterKernel<8> : SortScatterKernel<11>;
+            const bool few = p.tile == kSortWarps * kFewPerWarp;
+            const auto count = few ? SortCountKernel<kFewPerWarp> : SortCountKernel<kManyPerWarp>;
+            const auto scatter = x.bins < 256 ? (few ? SortScatterKernel<8, kFewPerWarp> : SortScatterKernel<8, kManyPerWarp>)
+                                              : (few ? SortScatterKernel<11, kFewPerWarp> : SortScatterKernel<11, kManyPerWarp>);
             if (int rc = Ck(MostSmem(scatter, most), "sort_by_expert")) return rc;
-            if (int rc = Ck(LaunchAfter(SortCountKernel, p.tiles, kSortBlock, x.bins * sizeof(int), s, x, hist), "sort_by_expert")) return rc;
+            if (int rc = Ck(LaunchAfter(count, p.tiles, kSortBlock, x.bins * sizeof(int), s, x, hist), "sort_by_expert")) return rc;
             if (int rc = Ck(LaunchAfter(SortScanKernel, blocks, kScanBlock, 0, s, hist, x.bins, p.tiles, sums), "sort_by_expert")) return rc;
-            return Ck(LaunchAfter(scatter, p.tiles, kSortBlock, kTile * sizeof(int2) + x.bins * sizeof(int) + SortSmem(kSortWarps, x.bins), s, x, hist, sums, records_out, sorted_out, order, position, offsets_out), "sort_by_expert");
+            return Ck(LaunchAfter(scatter, p.tiles, kSortBlock, p.tile * sizeof(int2) + x.bins * sizeof(int) + SortSmem(kSortWarps, x.bins), s, x, hist, sums, records_out, sorted_out, order, position, offsets_out), "sort_by_expert");
         };
         if (p.passes == 1) return pass(a, nullptr, nullptr, offsets);
         a.mask = p.bins[0] - 1;
