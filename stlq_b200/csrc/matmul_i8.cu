@@ -39,6 +39,7 @@ namespace tc = stlq_b200::tc;
 constexpr int kChannels = 128;                       // channels of a CTA's tile (its share of the MMA's M)
 constexpr int kTileK = 128;                          // bytes of a 128-byte swizzle row
 constexpr uint32_t kWBytes = kChannels * kTileK;
+constexpr int kBoxRows = 32;                         // rows come in boxes of these where a tile has fewer than its height
 constexpr int kWriters = 8;                          // warps of the epilogue
 constexpr int kShare = kWriters / 4;                 // of them, those of a quarter of the TMEM lanes
 constexpr int kThreads = 64 + 32 * kWriters;         // warp 0 loads, warp 1 multiplies, the others write
@@ -52,7 +53,8 @@ enum Mode { kOne, kPair, kSplit };
 
 template <int kRows, Mode kMode, typename T>
 struct Shape {
-    static constexpr uint32_t kXBytes = (kMode == kPair ? kRows / 2 : kRows) * kTileK;
+    static constexpr int kXRows = kMode == kPair ? kRows / 2 : kRows;  // rows that a CTA holds of a full tile
+    static constexpr uint32_t kXBytes = kXRows * kTileK;
     static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
     // A writing warp takes this many rows of its 32 channels at a time, and lays them out for a TMA store, twice.
     static constexpr int kChunk = kMode != kSplit && kRows >= 128 ? 32 : 16;
@@ -134,7 +136,8 @@ __device__ __forceinline__ Tile FindTile(const MatmulArgs& a, const Segments& sg
 template <int kRows, Mode kMode, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     MatmulI8Kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
-                   const __grid_constant__ CUtensorMap to, const MatmulArgs a, int cluster) {
+                   const __grid_constant__ CUtensorMap tx_part, const __grid_constant__ CUtensorMap to, const MatmulArgs a,
+                   int cluster) {
     using S = Shape<kRows, kMode, T>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = smem_raw + ((1024 - (tc::SmemAddr(smem_raw) & 1023)) & 1023);
@@ -236,20 +239,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
             const int wrow = t.expert * a.n + t.channel0 + (kMode == kPair ? rank * kChannels : 0);
             const int xrow = t.row0 + (kMode == kPair ? rank * (columns(t) / 2) : 0);
+            // The last tile of a segment loads the rows that it has: it would take as long as a full one otherwise.
+            const int boxes = S::kXRows <= kBoxRows ? 1 : (columns(t) * S::kXRows / kRows + kBoxRows - 1) / kBoxRows;
+            const bool whole = S::kXRows <= kBoxRows || boxes * kBoxRows == S::kXRows;
+            const uint32_t bytes = kWBytes + (whole ? S::kXBytes : boxes * kBoxRows * kTileK);
             for (int kb = k_first; kb < k_last; ++kb) {
                 if (used >= S::kStages && !(ok = __all_sync(0xffffffffu, tc::MbarWait(&empty[s], parity, a.err, kWaitNs)))) break;
                 unsigned char* st = base + s * S::kStageBytes;
                 if (one) {
                     if constexpr (kMode == kPair) {
                         // The even CTA's barrier counts the bytes of both.
-                        if (rank == 0) tc::MbarArriveExpectTx(&full[s], 2 * S::kStageBytes);
+                        if (rank == 0) tc::MbarArriveExpectTx(&full[s], 2 * bytes);
                         const uint32_t bar = tc::ClusterAddr(&full[s], 0);
                         tc::TmaLoad2dPair(st, &tw, bar, kb * kTileK, wrow);
-                        tc::TmaLoad2dPair(st + kWBytes, &tx, bar, kb * kTileK, xrow);
+                        if (whole) tc::TmaLoad2dPair(st + kWBytes, &tx, bar, kb * kTileK, xrow);
+                        else
+                            for (int i = 0; i < boxes; ++i)
+                                tc::TmaLoad2dPair(st + kWBytes + i * kBoxRows * kTileK, &tx_part, bar, kb * kTileK, xrow + i * kBoxRows);
                     } else {
-                        tc::MbarArriveExpectTx(&full[s], S::kStageBytes);
+                        tc::MbarArriveExpectTx(&full[s], bytes);
                         tc::TmaLoad2d(st, &tw, &full[s], kb * kTileK, wrow);
-                        tc::TmaLoad2d(st + kWBytes, &tx, &full[s], kb * kTileK, xrow);
+                        if (whole) tc::TmaLoad2d(st + kWBytes, &tx, &full[s], kb * kTileK, xrow);
+                        else
+                            for (int i = 0; i < boxes; ++i)
+                                tc::TmaLoad2d(st + kWBytes + i * kBoxRows * kTileK, &tx_part, &full[s], kb * kTileK, xrow + i * kBoxRows);
                     }
                 }
                 __syncwarp();
@@ -561,9 +574,11 @@ int64_t LikelyRowTiles(const MatmulArgs& a, int height) {
 template <int kRows, Mode kMode, typename T>
 cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
     using S = Shape<kRows, kMode, T>;
-    CUtensorMap tw, tx, to{};
+    CUtensorMap tw, tx, tx_part{}, to{};
     if (!MakeMap(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.w, static_cast<int64_t>(a.experts) * a.n, a.kdim, o.ldw, kChannels, kTileK) ||
-        !MakeMap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.q, a.rows, a.kdim, o.ldq, kMode == kPair ? kRows / 2 : kRows, kTileK))
+        !MakeMap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.q, a.rows, a.kdim, o.ldq, S::kXRows, kTileK))
+        return cudaErrorInvalidValue;
+    if (S::kXRows > kBoxRows && !MakeMap(&tx_part, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.q, a.rows, a.kdim, o.ldq, kBoxRows, kTileK))
         return cudaErrorInvalidValue;
     constexpr auto kOutType = sizeof(T) == 4                       ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                               : std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -595,7 +610,7 @@ cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
     attr[1].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
     config.attrs = attr;
     config.numAttrs = kMode == kOne ? 1 : 2;
-    return cudaLaunchKernelEx(&config, kernel, tw, tx, to, a, cluster);
+    return cudaLaunchKernelEx(&config, kernel, tw, tx, tx_part, to, a, cluster);
 }
 
 template <typename T>
