@@ -408,8 +408,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             for (int j = 0; j < kChunk; ++j) lay[j * 32 + lane] = Out<T>(y[j]);
                             tc::FenceAsyncShared();
                             __syncwarp();
-                            if (one && c - lane < a.n) {
-                                tc::TmaStore2d(&to, lay, c - lane, t.row0 + c0, policy);
+                            // A chunk past the last channel makes an empty group: the wait above counts groups,
+                            // and without one it would let the next chunk into a slot that is still read.
+                            if (one) {
+                                if (c - lane < a.n) tc::TmaStore2d(&to, lay, c - lane, t.row0 + c0, policy);
                                 tc::BulkCommit();
                             }
                             slot ^= 1;

@@ -176,6 +176,19 @@ def test_matmul_i8(k, dtype, rows, n, kdim):
     check_product(y, q, s, w, ws, bias, dtype)
 
 
+@pytest.mark.parametrize("dtype,rows,n,kdim", [(torch.float32, 7147, 2000, 52), (torch.float32, 3467, 1724, 208), (torch.bfloat16, 9000, 1944, 64), (torch.bfloat16, 5000, 4200, 300)])
+def test_matmul_i8_every_time(k, dtype, rows, n, kdim):
+    """Many tiles a block, with the last channels' tile partly past the end: forty calls give the same bits, and the right ones."""
+    g = rng_for(17, rows, n)
+    q, w = randq(g, rows, kdim), randq(g, n, kdim)
+    s, ws, bias = torch.rand(rows, generator=g), torch.rand(n, generator=g) / 128 / kdim, randn(g, n)
+    args = [t.cuda() for t in (q, s, w, ws, bias)]
+    first = k.matmul_i8(*args, out_dtype=dtype)
+    check_product(first, q, s, w, ws, bias, dtype)
+    for _ in range(40):
+        assert torch.equal(k.matmul_i8(*args, out_dtype=dtype), first)
+
+
 def test_matmul_i8_longest_sum(k):
     """131,071 terms of (-128)^2 are 2^31 - 2^14: the sum stays below the end of 32 bits."""
     kdim = 131071
