@@ -92,8 +92,8 @@ __device__ __noinline__ int Quantise(float x, float amax, float down) {
 struct RowScale {
     float amax, down, r;
     bool finite;
-    bool some;  // the row has numbers other than zeros, and nothing else
-    bool fast;  // 16-bit rows: products decide every value
+    bool some;   // the row has numbers other than zeros, and nothing else
+    bool quick;  // and products decide its values
 };
 
 // The same for N values without the division, which bound the kernel (16,384 x 4,096 bfloat16: 90 us with
@@ -107,7 +107,15 @@ struct RowScale {
 //
 // 32-bit rows.  x r with r = 127 / amax differs from the rounded quotient by less than 4 roundings of a number up to
 // 127 (4 * 127 * 2^-24 < 3.1e-5), so it rounds to the same integer unless it is nearer than that to the middle
-// between two; a pack with such a value is divided, as are rows where r is infinite or NaN.
+// between two; a pack with such a value is divided.
+template <typename T, int N>
+__device__ __noinline__ Pack<int8_t, N> DividePack(Pack<T, N> x, float amax, float down) {
+    Pack<int8_t, N> q;
+#pragma unroll
+    for (int i = 0; i < N; ++i) q.v[i] = static_cast<int8_t>(Quantise(ToFloat(x.v[i]), amax, down));
+    return q;
+}
+
 template <typename T, int N>
 __device__ __forceinline__ Pack<int8_t, N> QuantisePack(const Pack<T, N>& x, const RowScale& s) {
     constexpr float kMagic = 12582912.0f;
@@ -120,10 +128,7 @@ __device__ __forceinline__ Pack<int8_t, N> QuantisePack(const Pack<T, N>& x, con
         if (sizeof(T) != 2) sure = sure && fabsf(fmaf(v, s.r, kMagic - t)) < 0.5f - 4e-5f;
         low[i] = __float_as_uint(t);
     }
-    if (sizeof(T) == 2 ? !s.fast : !sure) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) low[i] = static_cast<unsigned>(Quantise(ToFloat(x.v[i]), s.amax, s.down));
-    }
+    if (sizeof(T) != 2 && !sure) return DividePack(x, s.amax, s.down);
     Pack<int8_t, N> q;
     if constexpr (N % 4 == 0) {
         unsigned* w = reinterpret_cast<unsigned*>(&q);
@@ -145,10 +150,11 @@ __device__ __forceinline__ RowScale ScaleOf(unsigned int top) {
     s.finite = top < 0x7f800000u;
     s.some = s.finite && top != 0;
     s.down = s.amax > 1e36f ? 0.00390625f : 1.0f;
-    s.fast = false;
+    // Where 127 / amax and its products are ordinary numbers.
+    s.quick = s.some && s.amax >= 1e-30f && s.amax <= 1e30f;
     if constexpr (sizeof(T) == 2) {
         s.r = 127.0f * (1.0f + 9.5367431640625e-7f) * __fdividef(1.0f, s.amax);  // 1 + 2^-20
-        s.fast = s.amax >= 1e-30f && s.amax <= 1e30f && ((top & 0x7fffffu) | 0x800000u) % 127u != 0;
+        s.quick = s.quick && ((top & 0x7fffffu) | 0x800000u) % 127u != 0;
     } else {
         s.r = __fdiv_rn(127.0f, s.amax);
     }
@@ -177,10 +183,10 @@ __device__ __forceinline__ unsigned int LargestBits(const Pack<T, N>& x, unsigne
 // re-reads the rest.  What a thread does once a row (addresses, the maximum over the group, the scale) costs as
 // much as quantising some five packs, and instructions bound the kernel; so a thread takes four packs, from four
 // threads a row for 128 bfloat16 to 256 for 8,192.  Sixteen packs a thread cost too many registers (66 us), two leave
-// too much beside them (48 us).  16,384 x 4,096 bfloat16 take 43 us, 4.6 TB/s, 300,000 x 128 26 us, one row of 4,096
+// too much beside them (48 us).  16,384 x 4,096 bfloat16 take 36 us, 5.5 TB/s, 300,000 x 128 22 us, one row of 4,096
 // 1.6 us (with 256 threads and two packs each, as its latency counts).
 template <typename T, int N, int L, int kHold, bool kSpread>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, sizeof(T) == 2 ? 6 : 4)
     QuantizeRowsKernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int topk,
                        const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
                        int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
@@ -242,22 +248,28 @@ __global__ void __launch_bounds__(kBlock)
             }
         }
     };
-    Out held[kHold];
+    // The packs in registers, where products decide them; a row that is divided reads its packs again, in the loop
+    // below (a test inside for each pack, with the division beside it, cost 16,384 x 4,096 bfloat16 6 us of 44).
+    int from = 0;
+    if (rs.quick) {
+        Out held[kHold];
 #pragma unroll
-    for (int h = 0; h < kHold; ++h) held[h] = rs.some ? QuantisePack(hold[h], rs) : Out{};
-    spread([&](int64_t to, bool real_row) {
-        Out* qr = reinterpret_cast<Out*>(q + to * ldq) + at;
-        if (real_row && kHold * L <= full) {
+        for (int h = 0; h < kHold; ++h) held[h] = QuantisePack(hold[h], rs);
+        spread([&](int64_t to, bool real_row) {
+            Out* qr = reinterpret_cast<Out*>(q + to * ldq) + at;
+            if (real_row && kHold * L <= full) {
 #pragma unroll
-            for (int h = 0; h < kHold; ++h) qr[h * L] = held[h];
-        } else {
+                for (int h = 0; h < kHold; ++h) qr[h * L] = held[h];
+            } else {
 #pragma unroll
-            for (int h = 0; h < kHold; ++h)
-                if (at + h * L < full) qr[h * L] = real_row ? held[h] : Out{};
-        }
-    });
-    for (int c = kHold * L; c + at < full; c += L) {
-        const Out r = rs.some ? QuantisePack(packs[c], rs) : Out{};
+                for (int h = 0; h < kHold; ++h)
+                    if (at + h * L < full) qr[h * L] = real_row ? held[h] : Out{};
+            }
+        });
+        from = kHold * L;
+    }
+    for (int c = from; c + at < full; c += L) {
+        const Out r = rs.quick ? QuantisePack(packs[c], rs) : rs.some ? DividePack(packs[c], rs.amax, rs.down) : Out{};
         spread([&](int64_t to, bool real_row) { (reinterpret_cast<Out*>(q + to * ldq) + at)[c] = real_row ? r : Out{}; });
     }
     if (full * N < cols)
