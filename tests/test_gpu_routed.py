@@ -127,6 +127,21 @@ def test_quantize_ties_zeros_and_infinities(k, dtype):
     assert q[1, :3].tolist() == [127, 0, 2]
 
 
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 7), (torch.float16, 10)])
+def test_quantize_every_16_bit_quotient(k, dtype, bits):
+    """Every mantissa of a row's largest value against every value down to 2^-9 of it: all the quotients that 16-bit rows can have, ties
+    among them (the largest value's mantissa a multiple of 127, and half the largest value)."""
+    one = 1 << bits
+    top = torch.arange(one, 2 * one, dtype=torch.float64)  # the largest value's significand
+    below = torch.cat([torch.arange(one, 2 * one, dtype=torch.float64) * 2.0**-s for s in range(10)])
+    x = torch.where(below[None] <= top[:, None], below[None], -0.5 * below[None])
+    x = torch.cat([top[:, None], x], 1) / 64  # exact in both types
+    assert torch.equal(x.to(dtype).double(), x)
+    q, s = k.quantize_rows(x.to(dtype).cuda())
+    want = torch.round(127 * x / (top[:, None] / 64)).to(torch.int8)
+    assert torch.equal(q.cpu(), want)
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_quantize_strided_and_unaligned(k, dtype):
     x = randn(rng_for(2), 11, 203, dtype=dtype)
@@ -282,7 +297,8 @@ def test_matmul_i8_grouped_offsets_out_of_order(k):
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("tokens,topk,experts", [(1, 1, 1), (1, 8, 64), (5, 2, 3), (33, 1, 10), (1000, 4, 256), (512, 8, 1024), (4097, 1, 1025), (300, 64, 2000),
-                                                 (20000, 2, 128), (70000, 1, 16384), (9000, 1, 65536), (100, 1, 65536)])
+                                                 (20000, 2, 128), (70000, 1, 16384), (9000, 1, 65536), (100, 1, 65536),
+                                                 (16384, 1, 100), (16385, 1, 100), (303104, 1, 3000), (303105, 1, 500), (151553, 2, 1024), (400000, 1, 1025)])
 def test_sort_by_expert(k, dtype, tokens, topk, experts):
     ids = random_ids(rng_for(9, tokens, topk, experts), tokens, topk, experts, 0.1, dtype)
     check_route(k.sort_by_expert(ids.cuda(), experts), ids, experts)
