@@ -29,8 +29,11 @@
 
 namespace {
 
+using stlq_b200::Aligned;
+using stlq_b200::Bad;
 using stlq_b200::Ck;
 using stlq_b200::DeviceScope;
+using stlq_b200::Guard;
 using stlq_b200::LetLaterStart;
 using stlq_b200::SetError;
 using stlq_b200::WaitForEarlier;
@@ -672,8 +675,6 @@ cudaError_t Launch(const Operands& o, const MatmulArgs& a) {
     return LaunchAs<T>(o, a, mode, best_height, best_parts);
 }
 
-int Bad(const char* msg) { return SetError(STLQ_B200_EINVAL, msg); }
-bool Aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(to) == 0; }
 
 int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_scale, const int8_t* w, int64_t ldw,
            const float* w_scale, const float* bias, const int32_t* offsets, int experts, int64_t rows, int n, int kdim,
@@ -712,15 +713,6 @@ int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_sc
     if (out_dtype == STLQ_B200_F32) return Ck(Launch<float>(o, a), "matmul_i8");
     if (out_dtype == STLQ_B200_BF16) return Ck(Launch<__nv_bfloat16>(o, a), "matmul_i8");
     return Ck(Launch<__half>(o, a), "matmul_i8");
-}
-
-template <typename F>
-int Guard(F&& f) {
-    try {
-        return f();
-    } catch (...) {
-        return STLQ_B200_ENOMEM;  // the only thing that throws here is a message's memory
-    }
 }
 
 }  // namespace

@@ -125,18 +125,20 @@ int stlq_b200_kernels_create(int device, stlq_b200_kernels** out) {
 }
 
 int stlq_b200_kernels_sync(stlq_b200_kernels* k, void* stream) {
-    if (!k) return stlq_b200::SetError(STLQ_B200_EINVAL, "kernel-provider handle is null");
-    DeviceScope scope(k->device);
-    if (!scope.ok()) return stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    unsigned int flags = 0;
-    if (int rc = Ck(cudaMemcpyAsync(&flags, k->err.p, sizeof(flags), cudaMemcpyDeviceToHost, s), "error flag")) return rc;
-    if (int rc = Ck(cudaStreamSynchronize(s), "cudaStreamSynchronize")) return rc;
-    if (!flags) return 0;
-    if (int rc = Ck(cudaMemsetAsync(k->err.p, 0, sizeof(flags), s), "error flag")) return rc;
-    return stlq_b200::SetError(STLQ_B200_EDEVICE, flags & stlq_b200::kErrWaitTimeout
-                                                      ? "a kernel's bounded wait expired: its results are not valid"
-                                                      : "a kernel reported an internal error");
+    return stlq_b200::Guard([&] {
+        if (!k) return stlq_b200::SetError(STLQ_B200_EINVAL, "kernel-provider handle is null");
+        DeviceScope scope(k->device);
+        if (!scope.ok()) return stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        unsigned int flags = 0;
+        if (int rc = Ck(cudaMemcpyAsync(&flags, k->err.p, sizeof(flags), cudaMemcpyDeviceToHost, s), "error flag")) return rc;
+        if (int rc = Ck(cudaStreamSynchronize(s), "cudaStreamSynchronize")) return rc;
+        if (!flags) return 0;
+        if (int rc = Ck(cudaMemsetAsync(k->err.p, 0, sizeof(flags), s), "error flag")) return rc;
+        return stlq_b200::SetError(STLQ_B200_EDEVICE, flags & stlq_b200::kErrWaitTimeout
+                                                          ? "a kernel's bounded wait expired: its results are not valid"
+                                                          : "a kernel reported an internal error");
+    });
 }
 
 int stlq_b200_kernels_destroy(stlq_b200_kernels* k) {

@@ -21,6 +21,19 @@ inline int Ck(cudaError_t e, const char* what) {
                     (std::string(what) + ": " + cudaGetErrorString(e)).c_str());
 }
 
+inline int Bad(const char* msg) { return SetError(STLQ_B200_EINVAL, msg); }
+inline bool Aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(to) == 0; }
+
+// Runs an entry point's body: nothing is thrown across the C boundary.
+template <typename F>
+int Guard(F&& f) {
+    try {
+        return f();
+    } catch (...) {
+        return STLQ_B200_ENOMEM;  // the only thing that throws here is a message's memory
+    }
+}
+
 struct Scratch {
     void* p = nullptr;
     size_t bytes = 0;

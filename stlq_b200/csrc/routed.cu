@@ -19,8 +19,11 @@
 
 namespace {
 
+using stlq_b200::Aligned;
+using stlq_b200::Bad;
 using stlq_b200::Ck;
 using stlq_b200::DeviceScope;
+using stlq_b200::Guard;
 using stlq_b200::LaunchAfter;
 using stlq_b200::LetLaterStart;
 using stlq_b200::SetError;
@@ -771,8 +774,6 @@ __global__ void __launch_bounds__(kBlock, 4)
 
 bool IsFloat(int dtype) { return dtype == STLQ_B200_F32 || dtype == STLQ_B200_BF16 || dtype == STLQ_B200_F16; }
 int64_t SizeOf(int dtype) { return dtype == STLQ_B200_F32 ? 4 : 2; }
-bool Aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(to) == 0; }
-int Bad(const char* msg) { return SetError(STLQ_B200_EINVAL, msg); }
 
 // Sets a kernel's dynamic shared memory limit, once for each device.
 template <typename K>
@@ -790,15 +791,6 @@ cudaError_t MostSmem(K kernel, size_t bytes) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (e == cudaSuccess && used < 8) seen[used++] = {reinterpret_cast<const void*>(kernel), device};
     return e;
-}
-
-template <typename F>
-int Guard(F&& f) {
-    try {
-        return f();
-    } catch (...) {
-        return STLQ_B200_ENOMEM;  // the only thing that throws here is a message's memory
-    }
 }
 
 template <typename F>
