@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 2 ? 6 : 4)
 // A counting sort over `bins` digits, stable: a tile of keys per block, each of its warps ranking a
 // contiguous piece 32 keys at a time (a ballot for each bit of the digit gives the lanes that share it).  Up to
 // kOneBins - 1 experts it is one pass; above that two passes of half the key's bits each, from the low
-// digit to the high one.  A sort that fits one block is one launch; others take three a pass: count, scan
+// digit to the high one.  A sort of few pairs is one launch of one block; others take three a pass: count, scan
 // each digit over the tiles, scatter.  12 bytes a pair are all that must move (2 us for a million): latency
 // bounds it, that of a launch (3.0 us for 512 pairs) or of seven with their barriers and, in the last, a scattered
 // write of each position (39 us for a million pairs over 16,384 experts; 9.4 us in three for 131,072 over 128).
@@ -303,8 +303,12 @@ constexpr int kFewPerWarp = 64, kManyPerWarp = 256;
 constexpr int64_t kFewPairs = 148 * kSortWarps * 2 * kFewPerWarp;
 constexpr int kOneBins = 1025;
 constexpr int kAloneBlock = 1024;
-constexpr int kAloneRounds = 16;                         // keys of a lane
-constexpr int kAlone = kAloneBlock * kAloneRounds;       // the most pairs of a sort by one block
+// The most pairs that one block sorts as fast as three launches (8,192 of 256 take it 14.1 us, three 10.5; 4,096 8.4), or over
+// two digits as seven (2,048 of 16,384 25 us, seven 20.9; 1,024 15.0): as many keys of a lane.
+constexpr int kAloneRounds = 4;
+constexpr int kAlone = kAloneBlock * kAloneRounds;
+constexpr int kWideRounds = 1;
+constexpr int kWide = kAloneBlock * kWideRounds;
 
 struct SortPass {
     const void* ids;   // first pass: the caller's ids
@@ -420,6 +424,78 @@ __global__ void __launch_bounds__(kAloneBlock)
     }
 }
 
+// A warp's part of the offsets of a two-pass sort: r is the first row of every expert after `after`, the key of row
+// r - 1, up to `to`, row r's.  The warp fills such a stretch together, as it may be as long as there are experts.
+__device__ __forceinline__ void FillOffsets(int r, int after, int to, int* __restrict__ offsets) {
+    const int lane = threadIdx.x & 31;
+    for (unsigned left = __ballot_sync(0xffffffffu, after < to); left; left &= left - 1) {
+        const int from = __ffs(left) - 1;
+        const int a = __shfl_sync(0xffffffffu, after, from), b = __shfl_sync(0xffffffffu, to, from);
+        for (int e = a + 1 + lane; e <= b; e += 32) offsets[e] = r - lane + from;
+    }
+}
+
+// Both passes of a sort over more than kOneBins - 1 experts in one block, the records between them in shared memory
+// (the seven launches of the general form take the host 20 us; this 10 to 15).
+template <int kBits>
+__global__ void __launch_bounds__(kAloneBlock)
+    SortWideKernel(SortPass a, SortPass b, int rounds, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
+    extern __shared__ int2 records[];  // [n], later the sorted keys; then base [bins] and the counts [warps][bins]
+    const int bins = max(a.bins, b.bins);
+    int* base = reinterpret_cast<int*>(records + a.n);
+    unsigned short* counts = reinterpret_cast<unsigned short*>(base + bins);
+    int* sorted = reinterpret_cast<int*>(records);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    LetLaterStart();
+    for (int i = threadIdx.x; i < warps * a.bins; i += blockDim.x) counts[i] = 0;
+    __syncthreads();
+    WaitForEarlier();
+    const int first = warp * rounds * 32 + lane;
+    int2 rec[kWideRounds];
+    unsigned short rank[kWideRounds];
+    // Each lane's place in the order of one digit.
+    auto pass = [&](const SortPass& p) {
+#pragma unroll
+        for (int r = 0; r < kWideRounds; ++r)
+            if (r < rounds)
+                rank[r] = static_cast<unsigned short>(CountRound<kBits>(
+                    first + r * 32 < a.n ? (rec[r].x >> p.shift) & p.mask : p.bins, p, counts + warp * p.bins));
+        __syncthreads();
+        ScanDigits(counts, warps, p.bins, base);
+    };
+    auto place = [&](const SortPass& p, int r) {
+        const int d = (rec[r].x >> p.shift) & p.mask;
+        return base[d] + counts[warp * p.bins + d] + rank[r];
+    };
+#pragma unroll
+    for (int r = 0; r < kWideRounds; ++r)
+        rec[r] = r < rounds && first + r * 32 < a.n ? make_int2(KeyOf(a, first + r * 32), first + r * 32) : make_int2(0, 0);
+    pass(a);
+#pragma unroll
+    for (int r = 0; r < kWideRounds; ++r)
+        if (r < rounds && first + r * 32 < a.n) records[place(a, r)] = rec[r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < warps * b.bins; i += blockDim.x) counts[i] = 0;
+#pragma unroll
+    for (int r = 0; r < kWideRounds; ++r)
+        if (r < rounds && first + r * 32 < a.n) rec[r] = records[first + r * 32];
+    __syncthreads();
+    pass(b);
+#pragma unroll
+    for (int r = 0; r < kWideRounds; ++r)
+        if (r < rounds && first + r * 32 < a.n) {
+            const int to = place(b, r);
+            order[to] = rec[r].y;
+            position[rec[r].y] = to;
+            sorted[to] = rec[r].x;  // every record is in registers by now
+        }
+    __syncthreads();
+    for (int r0 = warp * 32; r0 <= a.n; r0 += blockDim.x) {
+        const int r = r0 + lane;
+        FillOffsets(r, r <= a.n ? (r > 0 ? sorted[r - 1] : -1) : 0, r < a.n ? sorted[r] : r == a.n ? a.experts : -1, offsets);
+    }
+}
+
 // hist[b * tiles + tile] = keys of digit b in the tile.
 template <int kPerWarp>
 __global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* __restrict__ hist) {
@@ -472,23 +548,12 @@ __global__ void __launch_bounds__(kScanBlock) SortScanKernel(int* __restrict__ h
     if (lane == 0) sums[b] = carry;
 }
 
-// offsets of a two-pass sort: r is the first row of every expert after the key of row r - 1, up to row r's.
-// A warp fills such a stretch together, as it may be as long as there are experts.
+// offsets of a two-pass sort from its sorted keys.
 __global__ void SortOffsetsKernel(const int* __restrict__ sorted, int n, int experts, int* __restrict__ offsets) {
     LetLaterStart();
     WaitForEarlier();
-    const int lane = threadIdx.x & 31;
     const int r = blockIdx.x * blockDim.x + threadIdx.x;
-    int after = 0, to = -1;
-    if (r <= n) {
-        after = r > 0 ? sorted[r - 1] : -1;
-        to = r < n ? sorted[r] : experts;
-    }
-    for (unsigned left = __ballot_sync(0xffffffffu, after < to); left; left &= left - 1) {
-        const int from = __ffs(left) - 1;
-        const int a = __shfl_sync(0xffffffffu, after, from), b = __shfl_sync(0xffffffffu, to, from);
-        for (int e = a + 1 + lane; e <= b; e += 32) offsets[e] = r - lane + from;
-    }
+    FillOffsets(r, r <= n ? (r > 0 ? sorted[r - 1] : -1) : 0, r < n ? sorted[r] : r == n ? experts : -1, offsets);
 }
 
 // Each key to its place: the first of two passes writes records, the last one the order, the positions and
@@ -579,11 +644,10 @@ struct SortPlan {
     size_t sums, records, sorted, bytes;  // places in the workspace, which begins with the counts of each tile
 };
 
-bool Alone(int64_t n, int experts) { return n <= kAlone && experts + 1 <= kOneBins; }
+bool Alone(int64_t n, int experts) { return n <= (experts + 1 <= kOneBins ? kAlone : kWide); }
 
 SortPlan PlanSort(int64_t n, int experts) {
     SortPlan p{};
-    if (Alone(n, experts)) return p;
     p.tile = kSortWarps * (n <= kFewPairs ? kFewPerWarp : kManyPerWarp);
     p.tiles = static_cast<int>((n + p.tile - 1) / p.tile);
     if (experts + 1 <= kOneBins) {
@@ -597,6 +661,7 @@ SortPlan PlanSort(int64_t n, int experts) {
         p.bins[0] = 1 << p.shift[1];
         p.bins[1] = (experts >> p.shift[1]) + 1;
     }
+    if (Alone(n, experts)) return p;  // no workspace
     const auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     const size_t most = std::max(p.bins[0], p.bins[1]);
     p.sums = up(most * p.tiles * sizeof(int));
@@ -936,9 +1001,18 @@ int stlq_b200_sort_by_expert(stlq_b200_kernels* k, const void* ids, int ids_dtyp
         SortPass a{ids, ids_dtype == STLQ_B200_I64, nullptr, n, experts, 0, 0x7fffffff, experts + 1, p.tiles};
         const size_t most = 76 << 10;
         if (Alone(n, experts)) {
-            // As many warps as there are rounds for, so that few pairs take one round.
-            const int warps = std::min(kAloneBlock / 32, (n + 31) / 32);
+            // As many warps as there are rounds for, so that few pairs take one round, and not too few for the digits.
+            const int digits = std::max(p.bins[0], p.bins[1]);
+            const int warps = std::min(kAloneBlock / 32, std::max((n + 31) / 32, (digits + 127) / 128));
             const int rounds = (n + warps * 32 - 1) / (warps * 32);
+            if (p.passes == 2) {
+                a.bins = p.bins[0];
+                a.mask = p.bins[0] - 1;
+                const SortPass b{nullptr, 0, nullptr, n, experts, p.shift[1], 0x7fffffff, p.bins[1], 0};
+                const auto kernel = digits < 256 ? SortWideKernel<8> : SortWideKernel<11>;
+                if (int rc = Ck(MostSmem(kernel, 112 << 10), "sort_by_expert")) return rc;
+                return Ck(LaunchAfter(kernel, 1, warps * 32, n * sizeof(int2) + SortSmem(warps, digits), s, a, b, rounds, order, position, offsets), "sort_by_expert");
+            }
             const auto kernel = a.bins < 256 ? SortAloneKernel<8> : SortAloneKernel<11>;
             if (int rc = Ck(MostSmem(kernel, most), "sort_by_expert")) return rc;
             return Ck(LaunchAfter(kernel, 1, warps * 32, SortSmem(warps, a.bins), s, a, rounds, order, position, offsets), "sort_by_expert");

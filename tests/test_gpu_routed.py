@@ -298,15 +298,17 @@ def test_matmul_i8_grouped_offsets_out_of_order(k):
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("tokens,topk,experts", [(1, 1, 1), (1, 8, 64), (5, 2, 3), (33, 1, 10), (1000, 4, 256), (512, 8, 1024), (4097, 1, 1025), (300, 64, 2000),
                                                  (20000, 2, 128), (70000, 1, 16384), (9000, 1, 65536), (100, 1, 65536),
-                                                 (16384, 1, 100), (16385, 1, 100), (303104, 1, 3000), (303105, 1, 500), (151553, 2, 1024), (400000, 1, 1025)])
+                                                 (16384, 1, 100), (16385, 1, 100), (303104, 1, 3000), (303105, 1, 500), (151553, 2, 1024), (400000, 1, 1025),
+                                                 (1024, 1, 65536), (1025, 1, 65536), (512, 2, 1025), (31, 1, 1025), (200, 4, 5000), (1, 2, 30000), (777, 1, 16384),
+                                                 (4096, 1, 300), (4097, 1, 300), (500, 8, 1024), (2000, 2, 64)])
 def test_sort_by_expert(k, dtype, tokens, topk, experts):
     ids = random_ids(rng_for(9, tokens, topk, experts), tokens, topk, experts, 0.1, dtype)
     check_route(k.sort_by_expert(ids.cuda(), experts), ids, experts)
 
 
+@pytest.mark.parametrize("n", [10000, 4000, 1000])
 @pytest.mark.parametrize("experts", [1, 300, 5000])
-def test_sort_extreme_choices(k, experts):
-    n = 10000
+def test_sort_extreme_choices(k, experts, n):
     for fill in (0, experts - 1, experts, -1):
         ids = torch.full((n, 1), fill)
         check_route(k.sort_by_expert(ids.cuda(), experts), ids, experts)
