@@ -9,6 +9,7 @@
 // results do not change from call to call.
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -865,6 +866,19 @@ void ForType(int dtype, F&& f) {
     else f(__half{});
 }
 
+// The widest pack of T that the bases and row strides allow: 16 bytes, 8, 4, or one element.  An odd number of 16-bit
+// columns leaves one element a pack, which takes 2.4 times as long as 16 bytes (gradient of 16,384 x 4 x 2,047).
+template <typename T, typename F>
+void ForWidth(std::initializer_list<const void*> bases, std::initializer_list<int64_t> strides, F&& f) {
+    uint64_t all = 16;
+    for (const void* p : bases) all |= reinterpret_cast<uintptr_t>(p);
+    for (const int64_t v : strides) all |= static_cast<uint64_t>(v) * sizeof(T);
+    if (all % 16 == 0) f(std::integral_constant<int, 16 / sizeof(T)>{});
+    else if (all % 8 == 0) f(std::integral_constant<int, 8 / sizeof(T)>{});
+    else if (sizeof(T) == 2 && all % 4 == 0) f(std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 1>{});
+}
+
 // Threads per row: a warp for short rows, otherwise enough that a thread has at most `each` packs of it; more where
 // there are few rows, up to one pack a thread, as the time that one row takes is then the call's.
 template <typename F>
@@ -907,42 +921,48 @@ int Quantize(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int6
     cudaError_t error = cudaSuccess;
     ForType(x_dtype, [&](auto one) {
         using T = decltype(one);
-        constexpr int N = 16 / sizeof(T);
         const T* xp = static_cast<const T*>(x);
-        const bool wide = Aligned(x, 16) && ldx % N == 0 && Aligned(q, N) && ldq % N == 0;
-        const auto launch = [&](auto kernel, int L) {
-            const unsigned grid = Blocks(rows, L);
-            fits = grid != 0;
-            if (fits) error = LaunchAfter(kernel, grid, kBlock, 0, s, xp, ldx, rows, cols, topk, position, offsets, experts, pairs, q, ldq, scale);
-        };
-        const auto lay = [&](auto lanes, auto held) {
-            constexpr int L = decltype(lanes)::value, H = decltype(held)::value;
-            if (position) launch(QuantizeRowsKernel<T, N, L, H, true>, L);
-            else launch(QuantizeRowsKernel<T, N, L, H, false>, L);
-        };
-        using std::integral_constant;
-        const int packs = cols / N;
-        if (!wide && cols <= 128) {
-            if (position) launch(QuantizeRowsKernel<T, 1, 32, 4, true>, 32);
-            else launch(QuantizeRowsKernel<T, 1, 32, 4, false>, 32);
-        } else if (!wide) {
-            if (position) launch(QuantizeRowsKernel<T, 1, 256, 4, true>, 256);
-            else launch(QuantizeRowsKernel<T, 1, 256, 4, false>, 256);
-        } else if (packs > 16 && rows * ((packs + 3) / 4) < 1024 * static_cast<int64_t>(k->num_sms)) {
-            // Few rows: the time of one counts.
-            if (packs <= 64) lay(integral_constant<int, 32>{}, integral_constant<int, 2>{});
-            else if (packs <= 128) lay(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-            else lay(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-        } else {
-            const integral_constant<int, 4> four;
-            if (packs <= 16) lay(integral_constant<int, 4>{}, four);
-            else if (packs <= 32) lay(integral_constant<int, 8>{}, four);
-            else if (packs <= 64) lay(integral_constant<int, 16>{}, four);
-            else if (packs <= 128) lay(integral_constant<int, 32>{}, four);
-            else if (packs <= 256) lay(integral_constant<int, 64>{}, four);
-            else if (packs <= 512) lay(integral_constant<int, 128>{}, four);
-            else lay(integral_constant<int, 256>{}, four);
-        }
+        // A pack of N values is N bytes of q, so q's alignment counts as x's does.
+        ForWidth<T>({x, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(q) * sizeof(T))}, {ldx, ldq}, [&](auto width) {
+            constexpr int N = decltype(width)::value;
+            using std::integral_constant;
+            const auto lay = [&](auto lanes, auto held) {
+                constexpr int L = decltype(lanes)::value, H = decltype(held)::value;
+                const unsigned grid = Blocks(rows, L);
+                fits = grid != 0;
+                const auto launch = [&](auto kernel) {
+                    error = LaunchAfter(kernel, grid, kBlock, 0, s, xp, ldx, rows, cols, topk, position, offsets, experts, pairs, q, ldq, scale);
+                };
+                if (!fits) return;
+                if (position) launch(QuantizeRowsKernel<T, N, L, H, true>);
+                else launch(QuantizeRowsKernel<T, N, L, H, false>);
+            };
+            const int packs = cols / N;
+            if constexpr (N * sizeof(T) != 16) {
+                const integral_constant<int, 4> four;
+                const integral_constant<int, N == 1 ? 8 : 4> most;  // single elements cost few registers
+                if (packs <= 128) lay(integral_constant<int, 32>{}, four);
+                else if (packs <= 256 && N == 1) lay(integral_constant<int, 32>{}, most);
+                else if (packs <= 512) lay(integral_constant<int, 128>{}, four);
+                else if (packs <= 1024) lay(integral_constant<int, 256>{}, four);
+                else lay(integral_constant<int, 256>{}, most);
+            } else if (packs > 16 && rows * ((packs + 3) / 4) < 1024 * static_cast<int64_t>(k->num_sms)) {
+                // Few rows: the time of one counts.
+                const integral_constant<int, 2> two;
+                if (packs <= 64) lay(integral_constant<int, 32>{}, two);
+                else if (packs <= 128) lay(integral_constant<int, 64>{}, two);
+                else lay(integral_constant<int, 256>{}, two);
+            } else {
+                const integral_constant<int, 4> four;
+                if (packs <= 16) lay(integral_constant<int, 4>{}, four);
+                else if (packs <= 32) lay(integral_constant<int, 8>{}, four);
+                else if (packs <= 64) lay(integral_constant<int, 16>{}, four);
+                else if (packs <= 128) lay(integral_constant<int, 32>{}, four);
+                else if (packs <= 256) lay(integral_constant<int, 64>{}, four);
+                else if (packs <= 512) lay(integral_constant<int, 128>{}, four);
+                else lay(integral_constant<int, 256>{}, four);
+            }
+        });
     });
     if (!fits) return Bad("too many rows");
     return Ck(error, "quantize_rows");
@@ -1107,21 +1127,16 @@ int stlq_b200_combine(stlq_b200_kernels* k, const void* y, int dtype, int64_t ld
         cudaError_t error = cudaSuccess;
         ForType(dtype, [&](auto one) {
             using T = decltype(one);
-            constexpr int N = 16 / sizeof(T);
-            const bool wide = Aligned(y, 16) && ldy % N == 0 && Aligned(out, 16) && ldo % N == 0;
-            ForLanes(wide ? cols / N : cols, 4, tokens, k->num_sms, [&](auto lanes) {
-                constexpr int L = decltype(lanes)::value;
-                const unsigned grid = Blocks(tokens, L);
-                fits = grid != 0;
-                if (!fits) return;
-                const T* yp = static_cast<const T*>(y);
-                T* op = static_cast<T*>(out);
-                if (wide)
-                    error = LaunchAfter(CombineKernel<T, N, L>, grid, kBlock, 0, s, yp, ldy, tokens, cols, topk, weights, weights_dtype,
-                                                                   position, offsets, experts, pairs, op, ldo);
-                else
-                    error = LaunchAfter(CombineKernel<T, 1, L>, grid, kBlock, 0, s, yp, ldy, tokens, cols, topk, weights, weights_dtype,
-                                                                   position, offsets, experts, pairs, op, ldo);
+            ForWidth<T>({y, out}, {ldy, ldo}, [&](auto width) {
+                constexpr int N = decltype(width)::value;
+                ForLanes(cols / N, N * sizeof(T) == 16 ? 4 : 8, tokens, k->num_sms, [&](auto lanes) {
+                    constexpr int L = decltype(lanes)::value;
+                    const unsigned grid = Blocks(tokens, L);
+                    fits = grid != 0;
+                    if (fits)
+                        error = LaunchAfter(CombineKernel<T, N, L>, grid, kBlock, 0, s, static_cast<const T*>(y), ldy, tokens, cols, topk,
+                                            weights, weights_dtype, position, offsets, experts, pairs, static_cast<T*>(out), ldo);
+                });
             });
         });
         if (!fits) return Bad("too many tokens");
@@ -1152,23 +1167,17 @@ int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype
         cudaError_t error = cudaSuccess;
         ForType(dtype, [&](auto one) {
             using T = decltype(one);
-            constexpr int N = 16 / sizeof(T);
-            const bool wide = Aligned(dout, 16) && ldd % N == 0 && Aligned(y, 16) && ldy % N == 0 && Aligned(dy, 16) && lddy % N == 0;
-            ForLanes(wide ? cols / N : cols, 4, tokens, k->num_sms, [&](auto lanes) {
-                constexpr int L = decltype(lanes)::value;
-                const unsigned grid = Blocks(tokens, L);
-                fits = grid != 0;
-                if (!fits) return;
-                const T *dp = static_cast<const T*>(dout), *yp = static_cast<const T*>(y);
-                T* op = static_cast<T*>(dy);
-                if (wide)
-                    error = LaunchAfter(CombineBackwardKernel<T, N, L>, grid, kBlock, smem, s, dp, ldd, yp, ldy, tokens, cols, topk, weights,
-                                                                              weights_dtype, position, offsets, experts,
-                                                                              pairs, op, lddy, dweights);
-                else
-                    error = LaunchAfter(CombineBackwardKernel<T, 1, L>, grid, kBlock, smem, s, dp, ldd, yp, ldy, tokens, cols, topk, weights,
-                                                                              weights_dtype, position, offsets, experts,
-                                                                              pairs, op, lddy, dweights);
+            ForWidth<T>({dout, y, dy}, {ldd, ldy, lddy}, [&](auto width) {
+                constexpr int N = decltype(width)::value;
+                ForLanes(cols / N, N * sizeof(T) == 16 ? 4 : 8, tokens, k->num_sms, [&](auto lanes) {
+                    constexpr int L = decltype(lanes)::value;
+                    const unsigned grid = Blocks(tokens, L);
+                    fits = grid != 0;
+                    if (fits)
+                        error = LaunchAfter(CombineBackwardKernel<T, N, L>, grid, kBlock, smem, s, static_cast<const T*>(dout), ldd,
+                                            static_cast<const T*>(y), ldy, tokens, cols, topk, weights, weights_dtype, position, offsets,
+                                            experts, pairs, static_cast<T*>(dy), lddy, dweights);
+                });
             });
         });
         if (!fits) return Bad("too many tokens");

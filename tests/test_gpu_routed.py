@@ -100,7 +100,7 @@ def random_ids(g, tokens, topk, experts, drop=0.2, dtype=torch.int32):
 # ---- quantisation ------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 30), (9, 96), (33, 128), (2, 1000), (7, 960), (3, 4096), (2, 8200), (1, 20001)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 30), (9, 96), (33, 128), (2, 1000), (7, 960), (3, 4096), (2, 8200), (1, 20001), (9, 20), (5, 1004), (3, 2044), (700, 2047), (900, 254), (4, 2300)])
 def test_quantize_rows(k, dtype, rows, cols):
     x = randn(rng_for(1, rows, cols), rows, cols, dtype=dtype)
     q, s = k.quantize_rows(x.cuda())
@@ -322,7 +322,7 @@ def test_sort_extreme_choices(k, experts, n):
 # ---- exchange ----------------------------------------------------------------------------------
 
 EXCHANGE = [(1, 1, 1, 1, 0.0), (3, 2, 4, 30, 0.3), (50, 8, 16, 96, 0.1), (33, 4, 7, 200, 0.0), (20, 64, 100, 17, 0.2), (9, 2, 3, 1030, 0.5),
-            (130, 6, 8, 2048, 0.1), (5, 3, 2, 4104, 0.2), (40, 2, 5, 64, 1.0)]
+            (130, 6, 8, 2048, 0.1), (5, 3, 2, 4104, 0.2), (40, 2, 5, 64, 1.0), (40, 3, 6, 1004, 0.1), (21, 2, 4, 20, 0.2), (7, 5, 3, 2302, 0.1)]
 
 
 def setup_exchange(k, seed, tokens, topk, experts, cols, drop, dtype, wtype):
