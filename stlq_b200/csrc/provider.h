@@ -75,6 +75,9 @@ private:
 // in the stream ends.  Each such kernel calls WaitForEarlier before it touches global memory; that
 // returns when everything launched earlier in the stream has finished and is visible (each of these
 // kernels waits for the one before it), so the results are those of launches one after the other.
+// The kernel's life overlaps that of the launch that writes its inputs, so nothing in it may claim that
+// memory is read-only or its own while it runs: no __ldg and no __restrict__, whose loads the compiler may
+// fetch past the caches' order and move ahead of the wait.  Ordinary loads stay behind it.
 // LetLaterStart allows the next one to come up, which it does once every block has called it or left.
 __device__ __forceinline__ void WaitForEarlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void LetLaterStart() { asm volatile("griddepcontrol.launch_dependents;"); }

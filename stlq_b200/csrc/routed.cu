@@ -63,8 +63,12 @@ __device__ __forceinline__ void StoreStreaming(void* to, const P& v) {
 
 template <bool kStreaming, typename P>
 __device__ __forceinline__ void Load(P& v, const void* from) {
-    if constexpr (sizeof(P) == 16 && kStreaming) *reinterpret_cast<uint4*>(&v) = __ldcs(static_cast<const uint4*>(from));
-    else if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4*>(&v) = *static_cast<const uint4*>(from);
+    if constexpr (sizeof(P) == 16 && kStreaming) {
+        // Volatile, so that it stays behind WaitForEarlier.
+        uint4 u;
+        asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(from));
+        *reinterpret_cast<uint4*>(&v) = u;
+    } else if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4*>(&v) = *static_cast<const uint4*>(from);
     else v = *static_cast<const P*>(from);
 }
 
@@ -81,7 +85,7 @@ __device__ __forceinline__ void StoreAs(void* p, int64_t i, int dtype, float v) 
 
 // offsets[E] as the kernels use it: rows kept, within [0, P].
 __device__ __forceinline__ int Kept(const int* offsets, int experts, int pairs) {
-    return min(max(__ldg(offsets + experts), 0), pairs);
+    return min(max(offsets[experts], 0), pairs);
 }
 
 // ---- quantisation of rows ----------------------------------------------------------------------
@@ -191,9 +195,9 @@ __device__ __forceinline__ unsigned int LargestBits(const Pack<T, N>& x, unsigne
 // 1.6 us (with 256 threads and two packs each, as its latency counts).
 template <typename T, int N, int L, int kHold, bool kSpread>
 __global__ void __launch_bounds__(kBlock, sizeof(T) == 2 ? 6 : 4)
-    QuantizeRowsKernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int topk,
-                       const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
-                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
+    QuantizeRowsKernel(const T* x, int64_t ldx, int64_t rows, int cols, int topk,
+                       const int* position, const int* offsets, int experts, int pairs,
+                       int8_t* q, int64_t ldq, float* scale) {
     constexpr int kGroups = kBlock / L;
     using In = Pack<T, N>;
     using Out = Pack<int8_t, N>;
@@ -245,7 +249,7 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 2 ? 6 : 4)
             for (int j0 = 0; j0 < topk; j0 += 4) {  // four positions in flight
                 int p[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? __ldg(position + row * topk + j0 + j) : -1;
+                for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? position[row * topk + j0 + j] : -1;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (static_cast<unsigned>(p[j]) < static_cast<unsigned>(pairs)) write(static_cast<int64_t>(p[j]), p[j] < kept);
@@ -394,7 +398,7 @@ __device__ __forceinline__ void ScanDigits(unsigned short* counts, int warps, in
 // The whole sort in one block.
 template <int kBits>
 __global__ void __launch_bounds__(kAloneBlock)
-    SortAloneKernel(SortPass a, int rounds, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
+    SortAloneKernel(SortPass a, int rounds, int* order, int* position, int* offsets) {
     extern __shared__ int base[];  // [bins], then the counts [warps][bins]
     unsigned short* counts = reinterpret_cast<unsigned short*>(base + a.bins);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(kAloneBlock)
 
 // A warp's part of the offsets of a two-pass sort: r is the first row of every expert after `after`, the key of row
 // r - 1, up to `to`, row r's.  The warp fills such a stretch together, as it may be as long as there are experts.
-__device__ __forceinline__ void FillOffsets(int r, int after, int to, int* __restrict__ offsets) {
+__device__ __forceinline__ void FillOffsets(int r, int after, int to, int* offsets) {
     const int lane = threadIdx.x & 31;
     for (unsigned left = __ballot_sync(0xffffffffu, after < to); left; left &= left - 1) {
         const int from = __ffs(left) - 1;
@@ -440,7 +444,7 @@ __device__ __forceinline__ void FillOffsets(int r, int after, int to, int* __res
 // (the seven launches of the general form take the host 20 us; this 10 to 15).
 template <int kBits>
 __global__ void __launch_bounds__(kAloneBlock)
-    SortWideKernel(SortPass a, SortPass b, int rounds, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
+    SortWideKernel(SortPass a, SortPass b, int rounds, int* order, int* position, int* offsets) {
     extern __shared__ int2 records[];  // [n], later the sorted keys; then base [bins] and the counts [warps][bins]
     const int bins = max(a.bins, b.bins);
     int* base = reinterpret_cast<int*>(records + a.n);
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(kAloneBlock)
 
 // hist[b * tiles + tile] = keys of digit b in the tile.
 template <int kPerWarp>
-__global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* __restrict__ hist) {
+__global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* hist) {
     constexpr int kTile = kSortWarps * kPerWarp;
     extern __shared__ int base[];  // [bins]
     LetLaterStart();
@@ -519,7 +523,7 @@ __global__ void __launch_bounds__(kSortBlock) SortCountKernel(SortPass a, int* _
 
 // One warp per digit: its counts to the sums over the tiles before, its total to sums[].
 constexpr int kScanBlock = 256;
-__global__ void __launch_bounds__(kScanBlock) SortScanKernel(int* __restrict__ hist, int bins, int tiles, int* __restrict__ sums) {
+__global__ void __launch_bounds__(kScanBlock) SortScanKernel(int* hist, int bins, int tiles, int* sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     LetLaterStart();
     WaitForEarlier();
@@ -550,7 +554,7 @@ __global__ void __launch_bounds__(kScanBlock) SortScanKernel(int* __restrict__ h
 }
 
 // offsets of a two-pass sort from its sorted keys.
-__global__ void SortOffsetsKernel(const int* __restrict__ sorted, int n, int experts, int* __restrict__ offsets) {
+__global__ void SortOffsetsKernel(const int* sorted, int n, int experts, int* offsets) {
     LetLaterStart();
     WaitForEarlier();
     const int r = blockIdx.x * blockDim.x + threadIdx.x;
@@ -563,8 +567,8 @@ __global__ void SortOffsetsKernel(const int* __restrict__ sorted, int n, int exp
 // lay, a pass of a million took 27 us, most of them for partly filled sectors).
 template <int kBits, int kPerWarp>
 __global__ void __launch_bounds__(kSortBlock)
-    SortScatterKernel(SortPass a, const int* __restrict__ hist, const int* __restrict__ sums, int2* __restrict__ records,
-                      int* __restrict__ sorted, int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
+    SortScatterKernel(SortPass a, const int* hist, const int* sums, int2* records,
+                      int* sorted, int* order, int* position, int* offsets) {
     constexpr int kTile = kSortWarps * kPerWarp;
     extern __shared__ int2 tile[];  // [kTile], then the digits' places [2][bins] and the counts [kSortWarps][bins]
     __shared__ int part[32];
@@ -685,9 +689,9 @@ size_t SortSmem(int warps, int bins) { return static_cast<size_t>(bins) * 4 + st
 // (the copy rate measured is 6.54); 64 x 8 x 256 in 1.8 us.
 template <typename V, int L>
 __global__ void __launch_bounds__(kBlock)
-    DispatchKernel(const unsigned char* __restrict__ x, int64_t ldx, int64_t tokens, int packs, int topk,
-                   const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
-                   unsigned char* __restrict__ out, int64_t ldo) {
+    DispatchKernel(const unsigned char* x, int64_t ldx, int64_t tokens, int packs, int topk,
+                   const int* position, const int* offsets, int experts, int pairs,
+                   unsigned char* out, int64_t ldo) {
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + threadIdx.x / L;
     LetLaterStart();
     WaitForEarlier();
@@ -699,7 +703,7 @@ __global__ void __launch_bounds__(kBlock)
         for (int j0 = 0; j0 < topk; j0 += 4) {  // four positions in flight
             int p[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? __ldg(position + t * topk + j0 + j) : -1;
+            for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? position[t * topk + j0 + j] : -1;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (static_cast<unsigned>(p[j]) < static_cast<unsigned>(pairs))
@@ -714,9 +718,9 @@ __global__ void __launch_bounds__(kBlock)
 // 16,384 x 8 x 2,048 bfloat16 in 92 us, 6.5 TB/s; 64 x 8 x 256 in 2.4 us.
 template <typename T, int N, int L>
 __global__ void __launch_bounds__(kBlock)
-    CombineKernel(const T* __restrict__ y, int64_t ldy, int64_t tokens, int cols, int topk,
-                  const void* __restrict__ weights, int wtype, const int* __restrict__ position,
-                  const int* __restrict__ offsets, int experts, int pairs, T* __restrict__ out, int64_t ldo) {
+    CombineKernel(const T* y, int64_t ldy, int64_t tokens, int cols, int topk,
+                  const void* weights, int wtype, const int* position,
+                  const int* offsets, int experts, int pairs, T* out, int64_t ldo) {
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + threadIdx.x / L;
     LetLaterStart();
     WaitForEarlier();
@@ -733,7 +737,7 @@ __global__ void __launch_bounds__(kBlock)
             unsigned p[4];
             Pack<T, N> v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? static_cast<unsigned>(__ldg(position + t * topk + j0 + j)) : kept;
+            for (int j = 0; j < 4; ++j) p[j] = j0 + j < topk ? static_cast<unsigned>(position[t * topk + j0 + j]) : kept;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (p[j] < kept) Load<true>(v[j], y + p[j] * ldy + static_cast<int64_t>(c) * N);
@@ -753,7 +757,7 @@ __global__ void __launch_bounds__(kBlock)
     for (int c = full * N + threadIdx.x % L; c < cols; c += L) {
         float acc = 0.0f;
         for (int j = 0; j < topk; ++j) {
-            const unsigned p = static_cast<unsigned>(__ldg(position + t * topk + j));
+            const unsigned p = static_cast<unsigned>(position[t * topk + j]);
             if (p >= kept) continue;
             acc = fmaf(weights ? LoadAs(weights, t * topk + j, wtype) : 1.0f, ToFloat(y[p * ldy + c]), acc);
         }
@@ -767,10 +771,10 @@ __global__ void __launch_bounds__(kBlock)
 // 187 us, 6.5 TB/s; 64 x 8 x 256 in 4.0 us.
 template <typename T, int N, int L>
 __global__ void __launch_bounds__(kBlock, 4)
-    CombineBackwardKernel(const T* __restrict__ dout, int64_t ldd, const T* __restrict__ y, int64_t ldy, int64_t tokens,
-                          int cols, int topk, const void* __restrict__ weights, int wtype,
-                          const int* __restrict__ position, const int* __restrict__ offsets, int experts, int pairs,
-                          T* __restrict__ dy, int64_t lddy, void* __restrict__ dweights) {
+    CombineBackwardKernel(const T* dout, int64_t ldd, const T* y, int64_t ldy, int64_t tokens,
+                          int cols, int topk, const void* weights, int wtype,
+                          const int* position, const int* offsets, int experts, int pairs,
+                          T* dy, int64_t lddy, void* dweights) {
     extern __shared__ float part[];  // [kBlock / 32][topk]
     const int group = threadIdx.x / L, at = threadIdx.x % L, warp = threadIdx.x >> 5;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kBlock / L) + group;
@@ -786,7 +790,7 @@ __global__ void __launch_bounds__(kBlock, 4)
         float w[4], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            p[j] = real && j0 + j < topk ? __ldg(position + t * topk + j0 + j) : -1;
+            p[j] = real && j0 + j < topk ? position[t * topk + j0 + j] : -1;
             if (p[j] >= pairs) p[j] = -1;
             w[j] = p[j] >= 0 && p[j] < kept ? LoadAs(weights, t * topk + j0 + j, wtype) : 0.0f;
         }
