@@ -59,6 +59,7 @@ enum { STLQ_B200_F32 = 0, STLQ_B200_U8 = 1, STLQ_B200_BF16 = 2, STLQ_B200_F16 = 
 #define STLQ_B200_MAX_ROOT 65536 /* root codewords of a large-root encoder; experts of a sort or an exchange */
 #define STLQ_B200_MAX_TOPK 64     /* choices (experts) of one row */
 #define STLQ_B200_MAX_EXPERTS 1024 /* matrices of one grouped product */
+#define STLQ_B200_MAX_COLS 0x7ffff000 /* columns of a row that is quantised or exchanged: 2^31 - 4096 */
 #define STLQ_B200_MAX_I8_K 131071 /* terms of an 8-bit product's sum (a 32-bit integer holds it exactly) */
 
 /* Message for the last failed call on this host thread ("" if none). */
@@ -360,7 +361,8 @@ int stlq_b200_argmax_cols(stlq_b200_kernels* k, const float* scores, int ld, int
  * pointers are on the handle's device and aligned to their elements; calls are asynchronous on
  * `stream`, allocate nothing, keep nothing between calls and may be captured in a CUDA graph.  Outputs
  * must not overlap inputs.  "FLOAT" stands for STLQ_B200_F32, _BF16 or _F16.  A value is rounded to
- * a 16-bit type once, when it is written. */
+ * a 16-bit type once, when it is written.  A row that is quantised or exchanged has at most
+ * STLQ_B200_MAX_COLS columns. */
 
 /* q = the rows of x in 8 bits, scale = their scales: scale[r] = max_c |x[r, c]| / 127 and
  * q[r, c] = 127 x[r, c] / max_c |x[r, c]| rounded to the nearest integer (ties to even), both in 32 bits.  A row of

@@ -106,6 +106,13 @@ int64_t Rows(const Args& a, const char* name, const at::Tensor& t, bool type_ok,
     return ld;
 }
 
+// The same for rows that are quantised or exchanged.
+int64_t LongRows(const Args& a, const char* name, const at::Tensor& t, bool type_ok, const char* types) {
+    const int64_t ld = Rows(a, name, t, type_ok, types);
+    if (t.size(1) > STLQ_B200_MAX_COLS) throw Refused(std::string(name) + " has rows of more than 2^31 - 4096 elements");
+    return ld;
+}
+
 void Vector(const Args& a, const char* name, const at::Tensor& t, int64_t n, at::ScalarType type) {
     if (t.dim() != 1 || t.size(0) != n || t.scalar_type() != type || !t.is_contiguous())
         throw Refused(std::string(name) + " must be contiguous " + c10::toString(type) + " of shape (" + std::to_string(n) + ",), got " + Shown(t));
@@ -202,7 +209,7 @@ PyObject* QuantizeRows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return Guard([&] {
         const Args a(args, n, 3);
         const at::Tensor& x = a.Tensor(2, "x");
-        const int64_t ldx = Rows(a, "x", x, IsFloat(x.scalar_type()), kFloats);
+        const int64_t ldx = LongRows(a, "x", x, IsFloat(x.scalar_type()), kFloats);
         const int64_t rows = x.size(0), cols = x.size(1);
         const Rows8 q = Empty8(a, rows, cols);
         const at::Tensor scale = a.Empty({rows}, at::kFloat);
@@ -325,7 +332,7 @@ PyObject* Dispatch(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const Args a(args, n, 5);
         const at::Tensor& x = a.Tensor(2, "x");
         const int64_t size = x.element_size();
-        const int64_t ldx = Rows(a, "x", x, size == 1 || size == 2 || size == 4, "elements of 1, 2 or 4 bytes");
+        const int64_t ldx = LongRows(a, "x", x, size == 1 || size == 2 || size == 4, "elements of 1, 2 or 4 bytes");
         const Route r = Routing(a, 3);
         if (r.tokens != x.size(0)) throw Refused("the routing has " + std::to_string(r.tokens) + " rows, x " + std::to_string(x.size(0)));
         const int64_t cols = x.size(1);
@@ -342,7 +349,7 @@ PyObject* DispatchI8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return Guard([&] {
         const Args a(args, n, 5);
         const at::Tensor& x = a.Tensor(2, "x");
-        const int64_t ldx = Rows(a, "x", x, IsFloat(x.scalar_type()), kFloats);
+        const int64_t ldx = LongRows(a, "x", x, IsFloat(x.scalar_type()), kFloats);
         const Route r = Routing(a, 3);
         if (r.tokens != x.size(0)) throw Refused("the routing has " + std::to_string(r.tokens) + " rows, x " + std::to_string(x.size(0)));
         const int64_t cols = x.size(1);
@@ -362,7 +369,7 @@ PyObject* Combine(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const Args a(args, n, 6);
         const at::Tensor& y = a.Tensor(2, "y");
         const at::Tensor* w = a.Maybe(3, "weights");
-        const int64_t ldy = Rows(a, "y", y, IsFloat(y.scalar_type()), kFloats);
+        const int64_t ldy = LongRows(a, "y", y, IsFloat(y.scalar_type()), kFloats);
         const Route r = Routing(a, 4);
         if (y.size(0) != r.tokens * r.topk)
             throw Refused("y must have tokens * topk = " + std::to_string(r.tokens * r.topk) + " rows, got " + std::to_string(y.size(0)));
@@ -383,8 +390,8 @@ PyObject* CombineBackward(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const Args a(args, n, 7);
         const at::Tensor &dout = a.Tensor(2, "dout"), &y = a.Tensor(3, "y"), &w = a.Tensor(4, "weights");
         const Route r = Routing(a, 5);
-        const int64_t ldd = Rows(a, "dout", dout, IsFloat(dout.scalar_type()), kFloats);
-        const int64_t ldy = Rows(a, "y", y, y.scalar_type() == dout.scalar_type(), "dout's type");
+        const int64_t ldd = LongRows(a, "dout", dout, IsFloat(dout.scalar_type()), kFloats);
+        const int64_t ldy = LongRows(a, "y", y, y.scalar_type() == dout.scalar_type(), "dout's type");
         if (dout.size(0) != r.tokens || y.size(0) != r.tokens * r.topk || dout.size(1) != y.size(1))
             throw Refused("dout and y must have " + std::to_string(r.tokens) + " and " + std::to_string(r.tokens * r.topk) +
                           " rows of one length, got " + Shown(dout) + " and " + Shown(y));

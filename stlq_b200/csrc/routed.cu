@@ -32,6 +32,9 @@ using stlq_b200::WaitForEarlier;
 
 constexpr int kBlock = 256;
 constexpr int64_t kMostPairs = 0x7ffffc00;  // so that a block's worth past the last pair is still an int
+// Likewise for columns: a thread counts up to a row's packs, at most 8 of a block's worth ahead and one past the end.
+constexpr int kMostCols = STLQ_B200_MAX_COLS;
+static_assert(int64_t{kMostCols} + 8 * kBlock + 2 * kBlock <= 0x7fffffff, "a column counter past a row's end would overflow");
 
 template <typename T>
 __device__ __forceinline__ float ToFloat(T v) {
@@ -909,10 +912,17 @@ int CheckRouting(int64_t tokens, int topk, int experts, const void* position, co
     return 0;
 }
 
+int CheckCols(int64_t cols) {
+    if (cols < 0) return Bad("cols must be >= 0");
+    if (cols > kMostCols) return Bad("cols must be at most 2^31 - 4096");
+    return 0;
+}
+
 int Quantize(stlq_b200_kernels* k, const void* x, int x_dtype, int64_t ldx, int64_t rows, int cols, int topk,
              const int* position, const int* offsets, int experts, int8_t* q, int64_t ldq, float* scale, void* stream) {
     if (!IsFloat(x_dtype)) return Bad("x_dtype must be F32, BF16 or F16");
-    if (rows < 0 || cols < 0) return Bad("rows and cols must be >= 0");
+    if (rows < 0) return Bad("rows must be >= 0");
+    if (int rc = CheckCols(cols)) return rc;
     if (ldx < cols || ldq < cols) return Bad("ldx or ldq below cols");
     if (rows == 0) return 0;
     if (!scale || (cols > 0 && (!x || !q))) return Bad("null pointer");
@@ -1073,7 +1083,8 @@ int stlq_b200_dispatch(stlq_b200_kernels* k, const void* x, int elem_bytes, int6
         if (!k) return Bad("kernel-provider handle is null");
         if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return Bad("elem_bytes must be 1, 2 or 4");
         if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
-        if (cols < 0 || ldx < cols || ldo < cols) return Bad("cols >= 0, ldx >= cols and ldo >= cols required");
+        if (int rc = CheckCols(cols)) return rc;
+        if (ldx < cols || ldo < cols) return Bad("ldx and ldo must be at least cols");
         if (tokens == 0 || cols == 0) return 0;
         if (!x || !out) return Bad("null x or out");
         if (!Aligned(x, elem_bytes) || !Aligned(out, elem_bytes)) return Bad("x or out not aligned to its element");
@@ -1118,7 +1129,8 @@ int stlq_b200_combine(stlq_b200_kernels* k, const void* y, int dtype, int64_t ld
         if (!k) return Bad("kernel-provider handle is null");
         if (!IsFloat(dtype) || (weights && !IsFloat(weights_dtype))) return Bad("dtypes must be F32, BF16 or F16");
         if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
-        if (cols < 0 || ldy < cols || ldo < cols) return Bad("cols >= 0, ldy >= cols and ldo >= cols required");
+        if (int rc = CheckCols(cols)) return rc;
+        if (ldy < cols || ldo < cols) return Bad("ldy and ldo must be at least cols");
         if (tokens == 0 || cols == 0) return 0;
         if (!y || !out) return Bad("null y or out");
         if (!Aligned(y, SizeOf(dtype)) || !Aligned(out, SizeOf(dtype)) || (weights && !Aligned(weights, SizeOf(weights_dtype))))
@@ -1156,7 +1168,8 @@ int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype
         if (!k) return Bad("kernel-provider handle is null");
         if (!IsFloat(dtype) || !IsFloat(weights_dtype)) return Bad("dtypes must be F32, BF16 or F16");
         if (int rc = CheckRouting(tokens, topk, experts, position, offsets)) return rc;
-        if (cols < 0 || ldd < cols || ldy < cols || lddy < cols) return Bad("cols >= 0 and leading dimensions >= cols required");
+        if (int rc = CheckCols(cols)) return rc;
+        if (ldd < cols || ldy < cols || lddy < cols) return Bad("leading dimensions must be at least cols");
         if (tokens == 0) return 0;
         if (!weights || !dweights || (cols > 0 && (!dout || !y || !dy))) return Bad("null pointer");
         if (!Aligned(dout, SizeOf(dtype)) || !Aligned(y, SizeOf(dtype)) || !Aligned(dy, SizeOf(dtype)) ||
