@@ -380,7 +380,7 @@ int stlq_b200_matmul_i8(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, cons
 
 /* The same product where row r in [offsets[e], offsets[e + 1]) takes expert e's matrix: w (experts * n) x kdim,
  * expert e's channels at rows e n .. e n + n - 1, w_scale and bias likewise.  offsets: experts + 1 on the device, as
- * stlq_b200_sort_by_expert writes them.  Rows from offsets[experts] on are zeros. */
+ * stlq_b200_sort_by_expert writes them.  Rows before offsets[0] and from offsets[experts] on are zeros. */
 int stlq_b200_matmul_i8_grouped(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_scale, const int8_t* w,
                                 int64_t ldw, const float* w_scale, const float* bias, const int32_t* offsets, int experts,
                                 int64_t rows, int n, int kdim, void* out, int out_dtype, int64_t ldo, void* stream);

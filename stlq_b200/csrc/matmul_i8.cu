@@ -98,13 +98,50 @@ struct Tile {
 };
 
 // The segments of the experts, in shared memory: first[e] is the number of tiles before expert e's,
-// begin[e] / end[e] its rows, within the
-// product's.
+// begin[e] / end[e] its rows, within the product's.  Rows before begin[0] and from the last end on have no expert.
 struct Segments {
     int* first;
     int* begin;
     int* end;
 };
+
+// Fills sg from the offsets, by the kThreads threads of a block; `ct` tiles for every kRows rows or part of them.  The block
+// synchronises before it reads them.
+template <int kRows, int kThreads>
+__device__ __forceinline__ void FindSegments(const MatmulArgs& a, const Segments& sg, int ct) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int e = threadIdx.x; e < a.experts; e += kThreads) sg.end[e] = min(max(a.offsets[e + 1], 0), a.rows);
+    __syncthreads();
+    if (warp != 0) return;
+    int before = 0, top = min(max(a.offsets[0], 0), a.rows);
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+        const int e = e0 + lane;
+        // A segment begins where the one before it ended: a running maximum, so that offsets
+        // in any order give segments that do not overlap.
+        int end = e < a.experts ? sg.end[e] : 0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end = max(end, y);
+        }
+        end = max(end, top);
+        int begin = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) begin = top;
+        top = __shfl_sync(0xffffffffu, end, 31);
+        int s = e < a.experts ? (end - begin + kRows - 1) / kRows * ct : 0;
+        const int mine = s;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += y;
+        }
+        if (e < a.experts) {
+            sg.begin[e] = begin;
+            sg.end[e] = end;
+            sg.first[e] = before + s - mine;
+        }
+        before += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) sg.first[a.experts] = before;
+}
 
 template <int kRows, int kTileChannels>
 __device__ __forceinline__ Tile FindTile(const MatmulArgs& a, const Segments& sg, int id) {
@@ -183,40 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     LetLaterStart();
     WaitForEarlier();
-    if (a.offsets) {
-        for (int e = threadIdx.x; e < a.experts; e += kThreads) sg.end[e] = min(max(a.offsets[e + 1], 0), a.rows);
-        __syncthreads();
-        if (warp == 0) {
-            int before = 0, top = min(max(a.offsets[0], 0), a.rows);
-            for (int e0 = 0; e0 < a.experts; e0 += 32) {
-                const int e = e0 + lane;
-                // A segment begins where the one before it ended: a running maximum, so that offsets
-                // in any order give segments that do not overlap.
-                int end = e < a.experts ? sg.end[e] : 0;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, end, o);
-                    if (lane >= o) end = max(end, y);
-                }
-                end = max(end, top);
-                int begin = __shfl_up_sync(0xffffffffu, end, 1);
-                if (lane == 0) begin = top;
-                top = __shfl_sync(0xffffffffu, end, 31);
-                int s = e < a.experts ? (end - begin + kRows - 1) / kRows * ct : 0;
-                const int mine = s;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, s, o);
-                    if (lane >= o) s += y;
-                }
-                if (e < a.experts) {
-                    sg.begin[e] = begin;
-                    sg.end[e] = end;
-                    sg.first[e] = before + s - mine;
-                }
-                before += __shfl_sync(0xffffffffu, s, 31);
-            }
-            if (lane == 0) sg.first[a.experts] = before;
-        }
-    }
+    if (a.offsets) FindSegments<kRows, kThreads>(a, sg, ct);
     tc::FenceBeforeSync();
     if constexpr (kMode == kPair) {
         __syncthreads();
@@ -482,12 +486,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
-    if (a.offsets && warp >= 2) {  // rows after the last segment (dropped choices) hold zeros
+    if (a.offsets && warp >= 2) {  // rows without an expert (after the last segment: dropped choices) hold zeros
         T* out = static_cast<T*>(a.out);
-        const int64_t kept = sg.end[a.experts - 1];
-        const int64_t left = (a.rows - kept) * a.n;
-        for (int64_t i = static_cast<int64_t>(blockIdx.x) * (32 * kWriters) + threadIdx.x - 64; i < left; i += gridDim.x * (32 * kWriters))
-            out[(kept + i / a.n) * a.ldo + i % a.n] = Out<T>(0.0f);
+        const int64_t head = sg.begin[0], kept = sg.end[a.experts - 1];
+        const int64_t left = (head + a.rows - kept) * a.n;
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * (32 * kWriters) + threadIdx.x - 64; i < left; i += gridDim.x * (32 * kWriters)) {
+            const int64_t r = i / a.n;
+            out[(r < head ? r : kept + r - head) * a.ldo + i % a.n] = Out<T>(0.0f);
+        }
     }
     tc::FenceBeforeSync();
     __syncwarp();
@@ -499,27 +505,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Without a term to sum (kdim 0): the bias, and zeros after the last segment.
+// Without a term to sum (kdim 0): the bias, and zeros in rows without an expert.
+constexpr int kBiasBlock = 256;
 template <typename T>
-__global__ void BiasRowsKernel(const MatmulArgs a) {
+__global__ void __launch_bounds__(kBiasBlock) BiasRowsKernel(const MatmulArgs a) {
+    extern __shared__ int segments[];
+    Segments sg;
+    sg.first = segments;
+    sg.begin = sg.first + (a.experts + 1);
+    sg.end = sg.begin + a.experts;
     LetLaterStart();
     WaitForEarlier();
+    if (a.offsets) FindSegments<1, kBiasBlock>(a, sg, 0);
+    __syncthreads();
     const int64_t total = static_cast<int64_t>(a.rows) * a.n;
-    const int kept = a.offsets ? min(max(a.offsets[a.experts], 0), a.rows) : a.rows;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int head = a.offsets ? sg.begin[0] : 0, kept = a.offsets ? sg.end[a.experts - 1] : a.rows;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBiasBlock + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * kBiasBlock) {
         const int r = static_cast<int>(i / a.n), c = static_cast<int>(i % a.n);
         float y = 0.0f;
-        if (a.bias && r < kept) {
+        if (a.bias && r >= head && r < kept) {
             int e = 0;
             if (a.offsets) {
-                int lo = 0, hi = a.experts;
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (a.offsets[mid] <= r) lo = mid;
-                    else hi = mid;
+                int hi = a.experts - 1;  // the first expert whose segment ends after r
+                while (e < hi) {
+                    const int mid = (e + hi) >> 1;
+                    if (sg.end[mid] > r) hi = mid;
+                    else e = mid + 1;
                 }
-                e = lo;
             }
             y = a.bias[static_cast<int64_t>(e) * a.n + c];
         }
@@ -644,7 +657,7 @@ cudaError_t LaunchAs(const Operands& o, const MatmulArgs& a, Mode mode, int heig
 template <typename T>
 cudaError_t Launch(const Operands& o, const MatmulArgs& a) {
     if (a.kdim == 0) {
-        return stlq_b200::LaunchAfter(BiasRowsKernel<T>, o.sms * 4, 256, 0, o.stream, a);
+        return stlq_b200::LaunchAfter(BiasRowsKernel<T>, o.sms * 4, kBiasBlock, a.offsets ? (3 * static_cast<size_t>(a.experts) + 1) * 4 : 0, o.stream, a);
     }
     const int64_t ct = (a.n + kChannels - 1) / kChannels;
     const int nk = (a.kdim + kTileK - 1) / kTileK;

@@ -109,8 +109,8 @@ class Kernels:
 
     def matmul_i8_grouped(self, q, q_scale, w, w_scale, offsets, bias=None, out_dtype=None, out=None):
         """matmul_i8 with the matrix w[e] (n, cols) of the expert whose rows offsets[e] .. offsets[e + 1] - 1 are; w
-        (experts, n, cols), w_scale and bias (experts, n), offsets (experts + 1,) int32.  Rows from offsets[-1] on are
-        zeros.  At most 1,024 experts."""
+        (experts, n, cols), w_scale and bias (experts, n), offsets (experts + 1,) int32.  Rows before offsets[0] and from
+        offsets[-1] on are zeros.  At most 1,024 experts."""
         return self._ops.matmul_i8_grouped(self._h, self._d, q, q_scale, w, w_scale, offsets, bias, out_dtype, out)
 
     def sort_by_expert(self, ids, experts: int) -> Routing:

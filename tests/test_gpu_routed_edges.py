@@ -25,3 +25,36 @@ def test_rows_that_are_too_long(k):
     for call in (lambda: k.dispatch(x, r), lambda: k.dispatch_i8(h, r), lambda: k.quantize_rows(h), lambda: k.combine(h, w, r), lambda: k.combine_backward(h, h, w, r)):
         with pytest.raises(ValueError, match="2\\^31 - 4096"):
             call()
+
+
+# ---- segments ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kdim", [64, 0, 2048])
+@pytest.mark.parametrize("rows,n,first,last", [(25, 40, 3, 10), (25, 40, 25, 25), (700, 40, 300, 690), (3000, 600, 100, 2999)])
+def test_rows_before_the_first_segment_are_zeros(k, rows, n, first, last, kdim):
+    """An offset above 0 leaves rows without an expert in front, as the last one does behind: zeros in an output that held others."""
+    g = torch.Generator().manual_seed(rows + kdim)
+    q = torch.randint(-128, 128, (rows, kdim), generator=g).to(torch.int8)
+    w = torch.randint(-128, 128, (2, n, kdim), generator=g).to(torch.int8)
+    bias = torch.randint(1, 100, (2, n), generator=g).float()
+    out = torch.full((rows, n), 7.0, device="cuda")
+    middle = (first + last) // 2
+    offsets = torch.tensor([first, middle, last], dtype=torch.int32, device="cuda")
+    one = torch.ones(rows, device="cuda")
+    k.matmul_i8_grouped(q.cuda(), one, w.cuda(), torch.ones(2, n, device="cuda"), offsets, bias=bias.cuda(), out=out)
+    k.sync()
+    want = torch.zeros(rows, n, dtype=torch.float64)
+    for e, (a, b) in enumerate(((first, middle), (middle, last))):
+        want[a:b] = q[a:b].double() @ w[e].double().t() + bias[e]
+    # Whole numbers: in 32 bits the sum, which is at most |want| + 100, and the addition of the bias each round by 2^-24 at most.
+    assert ((out.double().cpu() - want).abs() <= 2.0**-23 * (want.abs() + 100)).all()
+    assert (out[:first] == 0).all() and (out[last:] == 0).all()
+
+
+@pytest.mark.parametrize("kdim", [64, 0])
+def test_offsets_out_of_order_give_the_same_segments_without_terms(k, kdim):
+    q, w = torch.zeros(50, kdim, dtype=torch.int8, device="cuda"), torch.zeros(4, 10, kdim, dtype=torch.int8, device="cuda")
+    bias = torch.arange(1.0, 5.0, device="cuda")[:, None].expand(4, 10).contiguous()
+    offsets = torch.tensor([-5, 30, 20, 2_000_000_000, 40], dtype=torch.int32, device="cuda")
+    y = k.matmul_i8_grouped(q, torch.ones(50, device="cuda"), w, torch.ones(4, 10, device="cuda"), offsets, bias=bias, out_dtype=torch.float32)
+    assert (y[:30] == 1).all() and (y[30:] == 3).all()
