@@ -420,8 +420,9 @@ int stlq_b200_combine_backward(stlq_b200_kernels* k, const void* dout, int dtype
                                const int32_t* position, const int32_t* offsets, int experts, void* dy, int64_t lddy,
                                void* dweights, void* stream);
 
-/* Waits for the work enqueued on `stream`; STLQ_B200_EDEVICE if a kernel of this handle reported an error since the
- * last call (a product whose bounded waits ran out). */
+/* Waits for the work enqueued on `stream`; STLQ_B200_EDEVICE if a kernel of this handle, on any stream, reported an error
+ * since the last call.  That is a product whose bounded waits ran out: its result is not valid, and no other call says so.
+ * Later calls are not affected. */
 int stlq_b200_kernels_sync(stlq_b200_kernels* k, void* stream);
 
 /* Block until all work this encoder enqueued on `stream` has finished; returns

@@ -71,6 +71,13 @@ struct Shape {
     static constexpr int kGranule = kMode == kPair ? 32 : 16;       // rows of an MMA come in multiples of this
 };
 
+// A wait that ran out raises *err, which stays raised until stlq_b200_kernels_sync reports it.  No wait gives up because it is
+// raised: it may be from an earlier call, and what that one lost would then cost later calls their results.  A block whose wait
+// ran out ends its loops, and whoever waits for it runs out in turn.
+__device__ __forceinline__ bool Wait(uint64_t* bar, uint32_t parity, unsigned int* err) {
+    return tc::MbarWait(bar, parity, err, kWaitNs, false);
+}
+
 struct MatmulArgs {
     const float* q_scale;
     const float* w_scale;
@@ -251,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool whole = S::kXRows <= kBoxRows || boxes * kBoxRows == S::kXRows;
             const uint32_t bytes = kWBytes + (whole ? S::kXBytes : boxes * kBoxRows * kTileK);
             for (int kb = k_first; kb < k_last; ++kb) {
-                if (used >= S::kStages && !(ok = __all_sync(0xffffffffu, tc::MbarWait(&empty[s], parity, a.err, kWaitNs)))) break;
+                if (used >= S::kStages && !(ok = __all_sync(0xffffffffu, Wait(&empty[s], parity, a.err)))) break;
                 unsigned char* st = base + s * S::kStageBytes;
                 if (one) {
                     if constexpr (kMode == kPair) {
@@ -287,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     s = S::kStages - 1;
                     parity ^= 1;
                 }
-                tc::MbarWait(&full[s], parity ^ 1, a.err, kWaitNs, false);
+                Wait(&full[s], parity ^ 1, a.err);
             }
         if (kMode == kPair && !ok) {  // the other CTA's barrier says no more: leave them 10 ms
             const uint64_t t0 = tc::GlobalTimerNs();
@@ -304,12 +311,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Tile t = FindTile<kRows, S::kTileChannels>(a, sg, id);
             const uint32_t idesc = tc::InstrDescI8(S::kTileChannels, columns(t));
             const int b = kMode == kSplit ? 0 : done & 1, use = done >> 1;
-            if (use > 0 && !(ok = __all_sync(0xffffffffu, tc::MbarWait(&taken[b], (use - 1) & 1, a.err, kWaitNs)))) break;
+            if (use > 0 && !(ok = __all_sync(0xffffffffu, Wait(&taken[b], (use - 1) & 1, a.err)))) break;
             tc::FenceAfterSync();
             const uint32_t acc = tmem + b * S::kColumns;
             uint32_t more = 0;
             for (int kb = k_first; kb < k_last; ++kb) {
-                if (!(ok = __all_sync(0xffffffffu, tc::MbarWait(&full[s], parity, a.err, kWaitNs)))) break;
+                if (!(ok = __all_sync(0xffffffffu, Wait(&full[s], parity, a.err)))) break;
                 tc::FenceAfterSync();
                 // Addresses in a descriptor count 16-byte units: a step of 32 bytes of kdim is 2.
                 const uint64_t dw = dw0 + s * (S::kStageBytes >> 4), dx = dx0 + s * (S::kStageBytes >> 4);
@@ -386,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (i * 32 + lane < S::kOwnRows) scales[i * 32 + lane] = now.qs[i];
             __syncwarp();
             T* direct = out + (static_cast<int64_t>(t.row0) + share * kChunk) * a.ldo + c;
-            ok = __all_sync(0xffffffffu, tc::MbarWait(&made[b], (done >> 1) & 1, a.err, kWaitNs));
+            ok = __all_sync(0xffffffffu, Wait(&made[b], (done >> 1) & 1, a.err));
             if (ok) {
                 tc::FenceAfterSync();
                 const uint32_t from = tmem + lanes + b * S::kColumns;

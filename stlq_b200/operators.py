@@ -152,7 +152,8 @@ class Kernels:
         return self._ops.combine_backward(self._h, self._d, dout, y, weights, routing.position, routing.offsets)
 
     def sync(self):
-        """Waits for the current stream; raises if a kernel of this handle reported an error."""
+        """Waits for the current stream; raises if a kernel of this handle, on any stream, reported an error since the last call:
+        a product whose bounded waits ran out, which nothing else reports and whose result is not valid."""
         import torch
 
         self._check(self._lib.stlq_b200_kernels_sync(ctypes.c_void_p(self._h), torch.cuda.current_stream(self._d).cuda_stream),

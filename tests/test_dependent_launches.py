@@ -39,3 +39,10 @@ def test_every_kernel_waits_once(name):
     """Each kernel of these files calls WaitForEarlier, so that 'everything earlier has finished' holds along a chain of launches."""
     bodies = re.split(r"\b__global__\b", code(name))[1:]
     assert bodies and all(b.split("__global__")[0].count("WaitForEarlier();") == 1 for b in bodies)
+
+
+def test_no_wait_of_the_products_gives_up_for_an_earlier_call():
+    """The handle's error word outlives a call.  A wait that gives up because the word is raised would spoil every later product until
+    someone asks for the error, so the products wait without looking at it (the last argument of MbarWait)."""
+    calls = re.findall(r"\bMbarWait\(([^;]*)\);", code("matmul_i8.cu"))
+    assert calls and all(c.rstrip().endswith(", false") for c in calls)
