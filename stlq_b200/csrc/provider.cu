@@ -91,6 +91,10 @@ __global__ void ArgmaxColsKernel(const float* __restrict__ scores, int64_t ld, i
     }
 }
 
+// Reads the error word and clears it in one step: a kernel on another stream may raise it at any time, and what it raises
+// after this is left for the next one to take.
+__global__ void TakeErrorsKernel(unsigned int* word, unsigned int* taken) { *taken = atomicExch(word, 0u); }
+
 int GridFor(int64_t total) { return static_cast<int>(std::min<int64_t>((total + 255) / 256, 148 * 32)); }
 
 }  // namespace
@@ -112,8 +116,8 @@ int stlq_b200_kernels_create(int device, stlq_b200_kernels** out) {
     DeviceScope scope(device);
     int rc = scope.ok() ? 0 : stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
     if (!rc) rc = Ck(cudaDeviceGetAttribute(&k->num_sms, cudaDevAttrMultiProcessorCount, device), "multiprocessor count");
-    if (!rc) rc = k->err.Ensure(sizeof(unsigned int));
-    if (!rc) rc = Ck(cudaMemset(k->err.p, 0, sizeof(unsigned int)), "cudaMemset");
+    if (!rc) rc = k->err.Ensure(2 * sizeof(unsigned int));
+    if (!rc) rc = Ck(cudaMemset(k->err.p, 0, k->err.bytes), "cudaMemset");
     if (!rc) rc = Ck(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize");  // before work on any other stream
     if (rc) {
         k->err.Release();
@@ -131,10 +135,14 @@ int stlq_b200_kernels_sync(stlq_b200_kernels* k, void* stream) {
         if (!scope.ok()) return stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         unsigned int flags = 0;
-        if (int rc = Ck(cudaMemcpyAsync(&flags, k->err.p, sizeof(flags), cudaMemcpyDeviceToHost, s), "error flag")) return rc;
+        unsigned int* word = static_cast<unsigned int*>(k->err.p);
+        cudaLaunchConfig_t one{};
+        one.gridDim = one.blockDim = dim3(1);
+        one.stream = s;
+        if (int rc = Ck(cudaLaunchKernelEx(&one, TakeErrorsKernel, word, word + 1), "error flag")) return rc;
+        if (int rc = Ck(cudaMemcpyAsync(&flags, word + 1, sizeof(flags), cudaMemcpyDeviceToHost, s), "error flag")) return rc;
         if (int rc = Ck(cudaStreamSynchronize(s), "cudaStreamSynchronize")) return rc;
         if (!flags) return 0;
-        if (int rc = Ck(cudaMemsetAsync(k->err.p, 0, sizeof(flags), s), "error flag")) return rc;
         return stlq_b200::SetError(STLQ_B200_EDEVICE, flags & stlq_b200::kErrWaitTimeout
                                                           ? "a kernel's bounded wait expired: its results are not valid"
                                                           : "a kernel reported an internal error");

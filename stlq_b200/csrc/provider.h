@@ -104,5 +104,5 @@ struct stlq_b200_kernels {
     int device = 0;
     int num_sms = 148;
     stlq_b200::Scratch At, Bt;  // op(A) rows / op(B) columns made contiguous when the operand layout needs it
-    stlq_b200::Scratch err;     // one word: kernels OR DeviceError bits into it (stlq_b200_kernels_sync reads it)
+    stlq_b200::Scratch err;     // kernels OR DeviceError bits into its first word; stlq_b200_kernels_sync takes them into its second
 };

@@ -46,3 +46,9 @@ def test_no_wait_of_the_products_gives_up_for_an_earlier_call():
     someone asks for the error, so the products wait without looking at it (the last argument of MbarWait)."""
     calls = re.findall(r"\bMbarWait\(([^;]*)\);", code("matmul_i8.cu"))
     assert calls and all(c.rstrip().endswith(", false") for c in calls)
+
+
+def test_errors_are_taken_in_one_step():
+    """A word that is read, waited for and cleared loses what a kernel on another stream raises in between."""
+    body = re.search(r"int stlq_b200_kernels_sync\(.*?\n}\n", code("provider.cu"), flags=re.S).group(0)
+    assert "cudaMemset" not in body and "atomicExch(word, 0u)" in code("provider.cu")
