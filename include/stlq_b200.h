@@ -328,7 +328,9 @@ int stlq_b200_encode_file_large_root(stlq_b200_encoder* enc, stlq_b200_reader* r
  * the reference's GPU backend seam; its CUDA implementation is src/core/kernel_provider_cuda_stream*
  * over cuBLAS).  The C++ provider class stlq::b200::B200StreamKernels
  * (stlq_b200/adapter/stlq_b200_kernels.h) implements that interface on them.  All pointers are on
- * the handle's device; work is enqueued on `stream` (NULL: the legacy default stream). */
+ * the handle's device; work is enqueued on `stream` (NULL: the legacy default stream).  A handle may be
+ * created while a stream is captured, and waits for nobody's work; it has to outlive the graphs that
+ * captured its calls. */
 typedef struct stlq_b200_kernels stlq_b200_kernels;
 int stlq_b200_kernels_create(int device, stlq_b200_kernels** out);
 int stlq_b200_kernels_destroy(stlq_b200_kernels* k);

@@ -95,6 +95,37 @@ __global__ void ArgmaxColsKernel(const float* __restrict__ scores, int64_t ld, i
 // after this is left for the next one to take.
 __global__ void TakeErrorsKernel(unsigned int* word, unsigned int* taken) { *taken = atomicExch(word, 0u); }
 
+// What allocates and frees for a handle neither belongs to a stream capture that is under way, in this thread or another, nor
+// breaks it.
+class OutsideCaptures {
+public:
+    OutsideCaptures() { ok_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+    ~OutsideCaptures() {
+        if (ok_) cudaThreadExchangeStreamCaptureMode(&mode_);
+    }
+
+private:
+    cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+    bool ok_ = false;
+};
+
+// The device's properties, and the error words at zero before work on any stream.  The copy has a stream of its own, so that
+// it waits for nobody's work.
+int SetUp(stlq_b200_kernels* k) {
+    stlq_b200::DeviceScope scope(k->device);
+    if (!scope.ok()) return stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
+    if (int rc = stlq_b200::Ck(cudaDeviceGetAttribute(&k->num_sms, cudaDevAttrMultiProcessorCount, k->device), "multiprocessor count")) return rc;
+    const OutsideCaptures outside;
+    const unsigned int zeros[2] = {0, 0};
+    if (int rc = k->err.Ensure(sizeof(zeros))) return rc;
+    cudaStream_t own = nullptr;
+    if (int rc = stlq_b200::Ck(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking), "cudaStreamCreate")) return rc;
+    cudaError_t e = cudaMemcpyAsync(k->err.p, zeros, sizeof(zeros), cudaMemcpyHostToDevice, own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+    const cudaError_t d = cudaStreamDestroy(own);
+    return stlq_b200::Ck(e != cudaSuccess ? e : d, "error word");
+}
+
 int GridFor(int64_t total) { return static_cast<int>(std::min<int64_t>((total + 255) / 256, 148 * 32)); }
 
 }  // namespace
@@ -105,27 +136,23 @@ using stlq_b200::DeviceScope;
 extern "C" {
 
 int stlq_b200_kernels_create(int device, stlq_b200_kernels** out) {
-    if (!out) return stlq_b200::SetError(STLQ_B200_EINVAL, "out is null");
-    *out = nullptr;
-    int ndev = 0;
-    if (int rc = Ck(cudaGetDeviceCount(&ndev), "cudaGetDeviceCount")) return rc;
-    if (device < 0 || device >= ndev) return stlq_b200::SetError(STLQ_B200_EINVAL, "device ordinal out of range");
-    auto* k = new (std::nothrow) stlq_b200_kernels();
-    if (!k) return stlq_b200::SetError(STLQ_B200_ENOMEM, "out of host memory");
-    k->device = device;
-    DeviceScope scope(device);
-    int rc = scope.ok() ? 0 : stlq_b200::SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
-    if (!rc) rc = Ck(cudaDeviceGetAttribute(&k->num_sms, cudaDevAttrMultiProcessorCount, device), "multiprocessor count");
-    if (!rc) rc = k->err.Ensure(2 * sizeof(unsigned int));
-    if (!rc) rc = Ck(cudaMemset(k->err.p, 0, k->err.bytes), "cudaMemset");
-    if (!rc) rc = Ck(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize");  // before work on any other stream
-    if (rc) {
-        k->err.Release();
-        delete k;
-        return rc;
-    }
-    *out = k;
-    return 0;
+    return stlq_b200::Guard([&] {
+        if (!out) return stlq_b200::SetError(STLQ_B200_EINVAL, "out is null");
+        *out = nullptr;
+        int ndev = 0;
+        if (int rc = Ck(cudaGetDeviceCount(&ndev), "cudaGetDeviceCount")) return rc;
+        if (device < 0 || device >= ndev) return stlq_b200::SetError(STLQ_B200_EINVAL, "device ordinal out of range");
+        auto* k = new (std::nothrow) stlq_b200_kernels();
+        if (!k) return stlq_b200::SetError(STLQ_B200_ENOMEM, "out of host memory");
+        k->device = device;
+        if (int rc = SetUp(k)) {
+            k->err.Release();
+            delete k;
+            return rc;
+        }
+        *out = k;
+        return 0;
+    });
 }
 
 int stlq_b200_kernels_sync(stlq_b200_kernels* k, void* stream) {
@@ -152,6 +179,7 @@ int stlq_b200_kernels_sync(stlq_b200_kernels* k, void* stream) {
 int stlq_b200_kernels_destroy(stlq_b200_kernels* k) {
     if (!k) return 0;
     DeviceScope scope(k->device);
+    const OutsideCaptures outside;
     k->At.Release();
     k->Bt.Release();
     k->err.Release();

@@ -58,3 +58,41 @@ def test_offsets_out_of_order_give_the_same_segments_without_terms(k, kdim):
     offsets = torch.tensor([-5, 30, 20, 2_000_000_000, 40], dtype=torch.int32, device="cuda")
     y = k.matmul_i8_grouped(q, torch.ones(50, device="cuda"), w, torch.ones(4, 10, device="cuda"), offsets, bias=bias, out_dtype=torch.float32)
     assert (y[:30] == 1).all() and (y[30:] == 3).all()
+
+
+# ---- the handle --------------------------------------------------------------------------------
+
+def test_a_new_handle_waits_for_no_work():
+    if not have_cuda():
+        pytest.skip("no CUDA device")
+    import stlq_b200
+
+    stlq_b200.Kernels(0).close()
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(2_000_000_000)  # a second or so on the default stream
+    done.record()
+    h = stlq_b200.Kernels(0)
+    assert not done.query()
+    h.close()
+    torch.cuda.synchronize()
+
+
+def test_a_handle_made_and_closed_during_a_capture(k):
+    import stlq_b200
+
+    x = torch.ones(4, device="cuda")
+    x + 1  # loaded before the capture
+    other = stlq_b200.Kernels(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = stlq_b200.Kernels(0)
+        other.close()
+        y = x + 1
+    graph.replay()
+    assert (y == 2).all()
+    q, s = h.quantize_rows(torch.ones(3, 16, device="cuda"))
+    assert (h.matmul_i8(q, s, q, s, out_dtype=torch.float32) - 16).abs().max() < 1e-4
+    h.sync()
+    h.close()
