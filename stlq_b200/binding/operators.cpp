@@ -7,6 +7,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -241,6 +242,8 @@ PyObject* Product(const Args& a, const at::Tensor& q, const at::Tensor& qs, cons
     if (out.dim() != 2 || out.size(0) != rows || out.size(1) != n)
         throw Refused("out must have shape (" + std::to_string(rows) + ", " + std::to_string(n) + "), got " + Shown(out));
     const int64_t ldo = Rows(a, "out", out, true, kFloats);
+    if (out.requires_grad() && c10::GradMode::is_enabled())
+        throw Refused("out requires a gradient, which this product does not have: detach it, or call under torch.no_grad()");
     int64_t ldq, ldw;
     const at::Tensor qo = Operand(a, "q", q, &ldq), wo = Operand(a, "w", w, &ldw);
     auto* h = static_cast<stlq_b200_kernels*>(a.handle);
@@ -255,6 +258,8 @@ PyObject* Product(const Args& a, const at::Tensor& q, const at::Tensor& qs, cons
                             ws.const_data_ptr<float>(), b, rows, static_cast<int>(n), static_cast<int>(kdim), out.mutable_data_ptr(),
                             FloatCode(kind), ldo, a.Stream()),
               "stlq_b200_matmul_i8");
+    // A backward pass that saved `out` has to see that it changed.
+    if (into != Py_None && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     return Wrap(out);
 }
 

@@ -103,7 +103,8 @@ class Kernels:
 
     def matmul_i8(self, q, q_scale, w, w_scale, bias=None, out_dtype=None, out=None):
         """q (rows, cols) times w (n, cols) transposed, both int8: (q w^T) q_scale[:, None] w_scale + bias, the sum exact,
-        rounded once to ``out_dtype`` (out's type, else bfloat16, unless said otherwise).  Operands whose rows do not begin
+        rounded once to ``out_dtype`` (out's type, else bfloat16, unless said otherwise).  ``out`` is written in place; it may
+        not require a gradient.  Operands whose rows do not begin
         on 16-byte boundaries are copied on every call: quantize_rows lays them out once."""
         return self._ops.matmul_i8(self._h, self._d, q, q_scale, w, w_scale, bias, out_dtype, out)
 

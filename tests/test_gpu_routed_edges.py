@@ -96,3 +96,41 @@ def test_a_handle_made_and_closed_during_a_capture(k):
     assert (h.matmul_i8(q, s, q, s, out_dtype=torch.float32) - 16).abs().max() < 1e-4
     h.sync()
     h.close()
+
+
+# ---- torch's autograd --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("grouped", [False, True])
+def test_out_counts_as_changed(k, grouped):
+    """A tensor that a backward pass saved and a product then overwrote is an error, not a wrong gradient."""
+    q, s = k.quantize_rows(torch.ones(4, 16, device="cuda"))
+    a = torch.ones(4, 4, device="cuda", requires_grad=True)
+    whole = torch.ones(4, 12, device="cuda")
+
+    def product(out):
+        if grouped:
+            return k.matmul_i8_grouped(q, s, q[None], s[None], torch.tensor([0, 4], dtype=torch.int32, device="cuda"), out=out)
+        return k.matmul_i8(q, s, q, s, out=out)
+
+    for out in (whole[:, :4], torch.ones(4, 4, device="cuda")):
+        loss = (a * out).sum()
+        assert product(out) is not None and out._version == 1
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    with torch.inference_mode():
+        held = torch.ones(4, 4, device="cuda")
+        product(held)
+    product(held)
+    assert (held - 16).abs().max() < 1e-4
+    assert product(None)._version == 0
+
+
+def test_out_that_requires_a_gradient(k):
+    q, s = k.quantize_rows(torch.ones(4, 16, device="cuda"))
+    out = torch.ones(4, 4, device="cuda", requires_grad=True)
+    for bad in (out, out * 1):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            k.matmul_i8(q, s, q, s, out=bad)
+    with torch.no_grad():
+        k.matmul_i8(q, s, q, s, out=out)
+    assert (out.detach() - 16).abs().max() < 1e-4
