@@ -171,34 +171,44 @@ def _functions():
         import torch
         from torch.autograd.function import once_differentiable
 
+        def save(ctx, kernels, routing, *tensors):
+            """Keeps the routing's arrays as saved tensors, so that a change to them before the backward pass is an error.
+            Arrays that were made in inference mode cannot be saved so, nor their changes be seen."""
+            arrays = (routing.position, routing.offsets)
+            ctx.kernels, ctx.untracked = kernels, arrays if any(t.is_inference() for t in arrays) else None
+            ctx.save_for_backward(*tensors, *(() if ctx.untracked else arrays))
+
+        def saved(ctx):
+            return ctx.kernels._ops, (ctx.kernels._h, ctx.kernels._d), (*ctx.saved_tensors, *(ctx.untracked or ()))
+
         class Dispatch(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, kernels, routing):
                 if not x.is_floating_point():
                     raise ValueError("only floating rows have a gradient")
-                ctx.kernels, ctx.routing = kernels, routing
+                save(ctx, kernels, routing)
                 return kernels.dispatch(x.detach(), routing)
 
             @staticmethod
             @once_differentiable
             def backward(ctx, dxs):
-                return ctx.kernels.dispatch_backward(dxs.contiguous(), ctx.routing), None, None
+                ops, handle, arrays = saved(ctx)
+                return ops.combine(*handle, dxs.contiguous(), None, *arrays), None, None
 
         class Combine(torch.autograd.Function):
             @staticmethod
             def forward(ctx, y, weights, kernels, routing):
-                ctx.kernels, ctx.routing, ctx.ones = kernels, routing, weights is None
-                ctx.save_for_backward(*((y,) if weights is None else (y, weights)))
-                return kernels.combine(y.detach(), None if weights is None else weights.detach(), routing)
+                ctx.ones = weights is None
+                save(ctx, kernels, routing, *(() if ctx.ones else (y, weights)))
+                return kernels.combine(y.detach(), None if ctx.ones else weights.detach(), routing)
 
             @staticmethod
             @once_differentiable
             def backward(ctx, dout):
-                dout, k, r = dout.contiguous(), ctx.kernels, ctx.routing
+                ops, handle, held = saved(ctx)
                 if ctx.ones:
-                    return k.dispatch(dout, r), None, None, None
-                y, weights = ctx.saved_tensors
-                dy, dweights = k.combine_backward(dout, y, weights, r)
+                    return ops.dispatch(*handle, dout.contiguous(), *held), None, None, None
+                dy, dweights = ops.combine_backward(*handle, dout.contiguous(), *held)
                 return dy, dweights, None, None
 
         _FUNCTIONS = Dispatch, Combine

@@ -134,3 +134,41 @@ def test_out_that_requires_a_gradient(k):
     with torch.no_grad():
         k.matmul_i8(q, s, q, s, out=out)
     assert (out.detach() - 16).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("which", ["position", "offsets"])
+@pytest.mark.parametrize("op", ["dispatch", "combine", "ones"])
+def test_a_routing_changed_before_the_backward_pass(k, op, which):
+    """The gradient goes along the arrays that the forward pass used; where they changed, it is an error, not a wrong gradient."""
+    ids, other = torch.tensor([[0], [1], [1]], device="cuda"), torch.tensor([[1], [-1], [0]], device="cuda")
+    r = k.sort_by_expert(ids, 2)
+    x = torch.ones(3, 4, device="cuda", requires_grad=True)
+
+    def forward():
+        if op == "dispatch":
+            return k.dispatch(x, r).sum()
+        return k.combine(x, torch.full((3, 1), 2.0, device="cuda") if op == "combine" else None, r).sum()
+
+    forward().backward()
+    assert (x.grad == (2 if op == "combine" else 1)).all()
+    loss = forward()
+    getattr(r, which).copy_(getattr(k.sort_by_expert(other, 2), which))
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    # Another array in its place is not a change to the one that was used.
+    x.grad = None
+    r = k.sort_by_expert(ids, 2)
+    loss = forward()
+    setattr(r, which, getattr(k.sort_by_expert(other, 2), which))
+    loss.backward()
+    assert (x.grad == (2 if op == "combine" else 1)).all()
+
+
+@pytest.mark.parametrize("op", ["dispatch", "combine"])
+def test_a_routing_made_in_inference_mode(k, op):
+    with torch.inference_mode():
+        r = k.sort_by_expert(torch.tensor([[0], [1], [-1]], device="cuda"), 2)
+    x = torch.ones(3, 4, device="cuda", requires_grad=True)
+    w = torch.ones(3, 1, device="cuda", requires_grad=True)
+    (k.dispatch(x, r) if op == "dispatch" else k.combine(x, w, r)).sum().backward()
+    assert x.grad.sum(1).tolist() == [4, 4, 0] and (op == "dispatch" or w.grad[:, 0].tolist() == [4, 4, 0])
