@@ -93,6 +93,8 @@ void On(const Args& a, const char* name, const at::Tensor& t) {
     if (!t.is_cuda() || t.get_device() != a.device)
         throw Refused(std::string(name) + " must be on cuda:" + std::to_string(a.device) + ", got " + t.device().str());
     if (t.layout() != at::kStrided) throw Refused(std::string(name) + " must be a dense tensor");
+    if (t._fw_grad(0).defined())  // it would be dropped without a word
+        throw Refused(std::string(name) + " carries a forward-mode tangent, and these operators have no forward-mode derivatives");
 }
 
 // A matrix with contiguous rows on the device; its leading dimension.

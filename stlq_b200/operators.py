@@ -6,6 +6,9 @@ Everything takes and returns CUDA tensors on the handle's device and runs on the
 what it allocates comes from torch's allocator on that stream.  Matrices are row-major; their rows may be strided, the
 elements of a row may not.  Wrong shapes, types, layouts or devices raise ValueError before anything is launched.
 
+``dispatch`` and ``combine`` have gradients.  The others have none and their results carry none, whatever their arguments
+require: they serve trained weights.  Forward-mode tangents are refused everywhere.
+
     k = stlq_b200.Kernels(device=0)
     wq, ws = k.quantize_rows(weights)                 # once, at load
     q, s = k.quantize_rows(x)

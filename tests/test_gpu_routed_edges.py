@@ -172,3 +172,28 @@ def test_a_routing_made_in_inference_mode(k, op):
     w = torch.ones(3, 1, device="cuda", requires_grad=True)
     (k.dispatch(x, r) if op == "dispatch" else k.combine(x, w, r)).sum().backward()
     assert x.grad.sum(1).tolist() == [4, 4, 0] and (op == "dispatch" or w.grad[:, 0].tolist() == [4, 4, 0])
+
+
+def test_forward_mode_is_refused(k):
+    """No operator has a forward-mode derivative; a tangent must not be lost silently."""
+    import torch.autograd.forward_ad as fwd
+
+    r = k.sort_by_expert(torch.tensor([[0], [1]], device="cuda"), 2)
+    x, one = torch.ones(2, 16, device="cuda"), torch.ones(2, device="cuda")
+    q, s = k.quantize_rows(x)
+    with fwd.dual_level():
+        d, v, w = fwd.make_dual(x, x), fwd.make_dual(one, one), fwd.make_dual(one[:, None], one[:, None])
+        for call in (lambda: k.dispatch(d, r), lambda: k.combine(d, None, r), lambda: k.combine(x, w, r), lambda: k.quantize_rows(d),
+                     lambda: k.dispatch_i8(d, r), lambda: k.matmul_i8(q, v, q, s), lambda: k.matmul_i8(q, s, q, s, bias=v),
+                     lambda: k.dispatch_backward(d, r), lambda: k.combine_backward(d, x, one[:, None], r)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        # A tensor that requires a gradient too goes to the autograd functions, which have no such rule either.
+        with pytest.raises((ValueError, RuntimeError)):
+            k.dispatch(fwd.make_dual(x.clone().requires_grad_(), x), r)
+        assert torch.equal(k.dispatch(x, r), x)  # ordinary tensors at a dual level
+    for transform in (lambda: torch.func.jvp(lambda t: k.dispatch(t, r), (x,), (x,)), lambda: torch.func.grad(lambda t: k.dispatch(t, r).sum())(x),
+                      lambda: torch.vmap(lambda t: k.dispatch(t, r))(x[None])):
+        with pytest.raises((ValueError, RuntimeError)):
+            transform()
+    assert torch.equal(k.dispatch(x, r), x)
