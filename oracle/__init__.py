@@ -198,12 +198,16 @@ class Oracle:
         return dict(B=B, a=a, cost=cost, xC=xC, xnorm2=xn, beam_sse=beam_sse, final_sse=final_sse)
 
 
+class ReferenceMissing(FileNotFoundError):
+    """The library of the reference's own functions was not built: its sources are not here."""
+
+
 class Reference:
     """The reference's own functions (compiled from its sources by oracle/Makefile)."""
 
     def __init__(self, path: str = REF_SO, threads: int | None = None):
         if not os.path.exists(path):
-            raise FileNotFoundError(f"{path} missing: build it with `make -C oracle ref` where the reference sources are")
+            raise ReferenceMissing(f"{path} missing: build it with `make -C oracle ref` where the reference sources are")
         self.lib = ctypes.CDLL(path)
         L = self.lib
         L.ref_precomp_create.restype = ctypes.c_void_p

@@ -15,6 +15,19 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200, sm_100a)")
 
 
+@pytest.hookimpl(wrapper=True)
+def pytest_runtest_call(item):
+    """A test that asks for the reference's own functions is skipped where their library is not built."""
+    try:
+        return (yield)
+    except FileNotFoundError as e:
+        import oracle
+
+        if isinstance(e, oracle.ReferenceMissing):
+            pytest.skip(str(e))
+        raise
+
+
 def golden_names():
     """Fixtures of the regular encode stage (EncodeBase)."""
     names = (os.path.splitext(os.path.basename(p))[0] for p in glob.glob(os.path.join(GOLDEN, "*.npz")))
