@@ -470,4 +470,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", "Checks and calls of 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__operators() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__operators() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "BUILT_FOR", STLQ_BUILT_FOR) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -60,20 +60,43 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return OUT
 
 
+def built_for() -> str:
+    """The torch and the Python that a binding built now is for; it shares C++ objects with the one and the ABI of the other."""
+    from importlib import metadata
+
+    try:
+        torch_version = metadata.version("torch")
+    except metadata.PackageNotFoundError:  # a torch that was not installed as a package
+        from torch import __version__ as torch_version
+    return f"torch {torch_version}, {sys.implementation.cache_tag}"
+
+
+def _read(path):
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> str:
     header = os.path.join(HERE, "..", "include", "stlq_b200.h")
-    if force or _stale(BINDING_OUT, [BINDING, header]):
+    os.makedirs(OBJDIR, exist_ok=True)
+    stamp = os.path.join(OBJDIR, "operators.for")
+    if force or _stale(BINDING_OUT, [BINDING, header]) or _read(stamp) != built_for():
         import importlib.util
 
         torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
         inc, lib = os.path.join(torch_dir, "include"), os.path.join(torch_dir, "lib")
         cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(NVCC))), "include")
-        cmd = [HOST_CXX, "-O2", "-std=c++17", "-shared", "-fPIC", BINDING, "-o", BINDING_OUT, "-I", inc, "-I",
+        cmd = [HOST_CXX, "-O2", "-std=c++17", "-shared", "-fPIC", f'-DSTLQ_BUILT_FOR="{built_for()}"', BINDING, "-o", BINDING_OUT, "-I", inc, "-I",
                os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_path("include"), "-I", cuda, "-L", lib,
                "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath," + lib]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+        with open(stamp, "w") as f:
+            f.write(built_for())
     return BINDING_OUT
 
 

@@ -36,11 +36,16 @@ def _ready():
 
         import torch  # noqa: F401  (the binding needs its libraries)
 
+        from . import build
+
         lib = load_library()
         try:
             ops = importlib.import_module("stlq_b200._operators")
         except ImportError as e:
             raise StlqB200Error(f"stlq_b200/_operators.so cannot be loaded ({e}): build it with `python -m stlq_b200.build`") from e
+        built, here = getattr(ops, "BUILT_FOR", "another version"), build.built_for()
+        if built != here:
+            raise StlqB200Error(f"stlq_b200/_operators.so was built for {built} and this is {here}: build it with `python -m stlq_b200.build`")
         v = ctypes.c_void_p
         lib.stlq_b200_kernels_create.argtypes = [ctypes.c_int, ctypes.POINTER(v)]
         lib.stlq_b200_kernels_destroy.argtypes = [v]
