@@ -104,17 +104,6 @@ __device__ __forceinline__ uint64_t CachePolicy(bool evict_first) {
     else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
     return p;
 }
-// Untiled copies: both addresses 16-byte aligned, a multiple of 16 bytes.
-__device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(SmemAddr(dst)),
-                 "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(SmemAddr(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void BulkStore(void* dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
-                 "r"(SmemAddr(src)), "r"(bytes)
-                 : "memory");
-}
 __device__ __forceinline__ void BulkCommit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // All but the last kLeft groups of this thread have read their shared memory.
 template <int kLeft>
