@@ -84,7 +84,7 @@ struct MatmulArgs {
     const float* bias;
     const int* offsets;  // null: one matrix, all rows
     int experts, rows, n, kdim;
-    int tma_out;         // the output's rows begin on 16-byte boundaries
+    int tma_n;           // channels that TMA may write: see Matmul
     int evict_first;     // the output is larger than the L2 cache's share for it
     int band;            // row tiles that run side by side over the channels
     void* out;
@@ -412,9 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             y[j + 2] = fmaf(__int2float_rn(v[j + 2]) * sc.z, ws, bias);
                             y[j + 3] = fmaf(__int2float_rn(v[j + 3]) * sc.w, ws, bias);
                         }
-                        // A chunk of this segment at once by TMA, which also leaves out what is past the
-                        // output's edges; rows that belong to the next segment are left out here.
-                        if (a.tma_out && (c0 + kChunk <= count || !a.offsets)) {
+                        // A chunk of this segment at once by TMA, which also leaves out rows past the output's
+                        // end; rows that belong to the next segment are left out here.
+                        if (c - lane < a.tma_n && (c0 + kChunk <= count || !a.offsets)) {
                             T* lay = reinterpret_cast<T*>(outs + (2 * (warp - 2) + slot) * S::kOutBytes);
                             if (one) tc::BulkWaitRead<1>();
                             __syncwarp();
@@ -422,10 +422,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             for (int j = 0; j < kChunk; ++j) lay[j * 32 + lane] = Out<T>(y[j]);
                             tc::FenceAsyncShared();
                             __syncwarp();
-                            // A chunk past the last channel makes an empty group: the wait above counts groups,
-                            // and without one it would let the next chunk into a slot that is still read.
+                            // Every chunk that takes a slot makes a group: the wait above counts groups.
                             if (one) {
-                                if (c - lane < a.n) tc::TmaStore2d(&to, lay, c - lane, t.row0 + c0, policy);
+                                tc::TmaStore2d(&to, lay, c - lane, t.row0 + c0, policy);
                                 tc::BulkCommit();
                             }
                             slot ^= 1;
@@ -608,7 +607,7 @@ cudaError_t LaunchTiles(const Operands& o, const MatmulArgs& a, int cluster) {
     constexpr auto kOutType = sizeof(T) == 4                       ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                               : std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (kMode != kSplit && a.tma_out &&
+    if (kMode != kSplit && a.tma_n > 0 &&
         !MakeMap(&to, kOutType, a.out, a.rows, a.n, a.ldo * static_cast<int64_t>(sizeof(T)), S::kChunk, 32))
         return cudaErrorInvalidValue;
     const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kAllOut + (2 * S::kStages + 4) * 8 + 16 +
@@ -719,15 +718,18 @@ int Matmul(stlq_b200_kernels* k, const int8_t* q, int64_t ldq, const float* q_sc
     DeviceScope scope(k->device);
     if (!scope.ok()) return SetError(STLQ_B200_ECUDA, "cudaSetDevice failed");
     const int64_t out_bytes = out_dtype == STLQ_B200_F32 ? 4 : 2;
-    // TMA's rows: on 16-byte boundaries, less than 2^40 bytes apart.
-    const int tma_out = Aligned(out, 16) && ldo * out_bytes % 16 == 0 && ldo < (int64_t{1} << 37);
+    // TMA's rows begin on 16-byte boundaries, less than 2^40 bytes apart.  It leaves out what is past a row's end in steps of 16
+    // bytes: an output whose rows end inside such a step, as one that is part of a wider matrix may, has the channels of
+    // its last, partial chunk written by the threads.
+    const bool tma = Aligned(out, 16) && ldo * out_bytes % 16 == 0 && ldo < (int64_t{1} << 37);
+    const int tma_n = !tma ? 0 : n * out_bytes % 16 == 0 ? n : n / 32 * 32;
     // A large output is written in rows as long as possible, and leaves the cache in that order: tiles run along
     // the channels and its lines are marked to go first (4,096 x 65,536 x 128 to 32 bits: 220 us without the two,
     // 205 with the mark, 166 with both, 6.5 TB/s).  A matrix that does not stay in the cache from one row of
     // tiles to the next is read for eight at a time instead.
     const int evict_first = static_cast<int64_t>(rows) * n * out_bytes > (int64_t{48} << 20);
     const int band = static_cast<int64_t>(n) * kdim <= (int64_t{32} << 20) ? 1 : 8;
-    const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, tma_out, evict_first, band, out, ldo,
+    const MatmulArgs a{q_scale, w_scale, bias, offsets, experts, static_cast<int>(rows), n, kdim, tma_n, evict_first, band, out, ldo,
                        static_cast<unsigned int*>(k->err.p)};
     const Operands o{q, ldq, w, ldw, k->num_sms, k->device, static_cast<cudaStream_t>(stream)};
     if (out_dtype == STLQ_B200_F32) return Ck(Launch<float>(o, a), "matmul_i8");

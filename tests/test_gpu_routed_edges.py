@@ -197,3 +197,39 @@ def test_forward_mode_is_refused(k):
         with pytest.raises((ValueError, RuntimeError)):
             transform()
     assert torch.equal(k.dispatch(x, r), x)
+
+
+# ---- outputs inside a wider matrix -------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,n,kdim,experts", [(40, 1, 32, 0), (40, 3, 32, 0), (300, 33, 32, 0), (300, 130, 48, 0), (1000, 255, 64, 0), (3000, 1001, 1490, 0),
+                                                 (300, 130, 48, 3), (9000, 130, 1500, 24), (3000, 513, 2500, 24)])
+def test_a_product_writes_its_own_channels_alone(k, dtype, rows, n, kdim, experts):
+    """The output's rows lie on 16-byte boundaries and end inside 16 bytes: what follows them in the matrix stays.  The rows of
+    both products (one form each of a CTA's own tiles and of pairs) are ones, so the values are exact."""
+    whole = torch.full((rows, (n + 7) // 8 * 8 + 8), 7.0, dtype=dtype, device="cuda")
+    out = whole[:, :n]
+    q, one = torch.ones(rows, kdim, dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda")
+    if experts:
+        w, ws = torch.ones(experts, n, kdim, dtype=torch.int8, device="cuda"), torch.full((experts, n), 1 / kdim, device="cuda")
+        offsets = torch.linspace(0, rows - 5, experts + 1).int().cuda()
+        k.matmul_i8_grouped(q, one, w, ws, offsets, out=out)
+        assert (out[-5:] == 0).all()
+        out = out[:-5]
+    else:
+        k.matmul_i8(q, one, torch.ones(n, kdim, dtype=torch.int8, device="cuda"), torch.full((n,), 1 / kdim, device="cuda"), out=out)
+    k.sync()
+    # kdim * (1 / kdim), two roundings in 32 bits: one in the quotient, one in the product.
+    assert ((out.double() - 1).abs() <= (2.0**-22 if dtype == torch.float32 else 2.0**-11 if dtype == torch.float16 else 2.0**-8)).all()
+    assert (whole[:, n:] == 7).all()
+
+
+def test_bytes_past_the_terms_are_not_used(k):
+    """Rows of 16-byte multiples whose last bytes are no terms: they hold anything."""
+    g = torch.Generator().manual_seed(3)
+    for rows, n, kdim in ((70, 90, 17), (300, 200, 129), (1500, 2000, 1490), (130, 130, 2501), (5, 5, 1)):
+        wide = (kdim + 15) // 16 * 16
+        q, w = (torch.randint(-128, 128, (m, wide), generator=g).to(torch.int8) for m in (rows, n))
+        y = k.matmul_i8(q.cuda()[:, :kdim], torch.ones(rows, device="cuda"), w.cuda()[:, :kdim], torch.ones(n, device="cuda"), out_dtype=torch.float32)
+        want = q[:, :kdim].double() @ w[:, :kdim].double().t()
+        assert ((y.double().cpu() - want).abs() <= 2.0**-24 * want.abs()).all()
