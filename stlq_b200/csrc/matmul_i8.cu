@@ -494,12 +494,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (a.offsets && warp >= 2) {  // rows without an expert (after the last segment: dropped choices) hold zeros
         T* out = static_cast<T*>(a.out);
-        const int64_t head = sg.begin[0], kept = sg.end[a.experts - 1];
-        const int64_t left = (head + a.rows - kept) * a.n;
-        for (int64_t i = static_cast<int64_t>(blockIdx.x) * (32 * kWriters) + threadIdx.x - 64; i < left; i += gridDim.x * (32 * kWriters)) {
-            const int64_t r = i / a.n;
-            out[(r < head ? r : kept + r - head) * a.ldo + i % a.n] = Out<T>(0.0f);
-        }
+        auto zeros = [&](int64_t from, int64_t to) {
+            const int64_t left = (to - from) * a.n;
+            for (int64_t i = static_cast<int64_t>(blockIdx.x) * (32 * kWriters) + threadIdx.x - 64; i < left; i += gridDim.x * (32 * kWriters))
+                out[(from + i / a.n) * a.ldo + i % a.n] = Out<T>(0.0f);
+        };
+        zeros(0, sg.begin[0]);
+        zeros(sg.end[a.experts - 1], a.rows);
     }
     tc::FenceBeforeSync();
     __syncwarp();
