@@ -11,10 +11,15 @@
 // What bounds it on B200 (2 x the measured bfloat16 rate is 3.37 POP/s, memory 6.54 TB/s):
 //   16,384 x 4,096 x 4,096    165 us, 3.33 POP/s: the tensor cores (78 % busy in a capture, at 1.6 GHz: power)
 //   4,096 x 65,536 x 128      168 us, 6.4 TB/s: writing 32-bit results
-//   1 x 4,096 x 4,096         6.5 us: what a launch, a cluster's sum and 2.6 us of weights take
-//   8 tokens x 8 of 128 experts, 1,024 x 2,048 each: 23 us, 4.7 TB/s of weights: three rounds of 2.76 tiles an SM
-//   32,768 rows over 64 experts, 2,048 x 2,048 each: 122 us (82 by the tensor cores, 72 by memory): both, and the
-//   last tile of each segment
+//   1 x 4,096 x 4,096         6.5 us: the latency of a launch and of a cluster's sum (2.6 us of weights, which stay in
+//   the L2 cache when calls repeat)
+//   8 tokens x 8 of 128 experts, 1,024 x 2,048 each: 23 us, 4.7 TB/s of weights; three rounds of 2.76 tiles an SM cost 8 %
+//   of it, the segments are found before the first load, the rest is not accounted for
+//   32,768 rows over 64 experts, 2,048 x 2,048 each: 122 to 127 us (82 by the tensor cores, 72 by memory).  Neither is
+//   busy throughout: in a capture of half the size the tensor cores work 57 % of the time and memory moves at 48 % of
+//   its rate; the last round of tiles costs 5 %, and tiles of 256 rows cover 23 % more rows than there are
+//   131,072 rows of 64 experts, 2,048 x 4,096 each: 809 us, and 1,371 when half of them have no expert: their zeros take a
+//   64-bit division an element, after the tiles
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -657,10 +662,12 @@ cudaError_t LaunchAs(const Operands& o, const MatmulArgs& a, Mode mode, int heig
 // 0.22 us + 0.4 ns h for every 128 terms (issuing the loads and MMAs bounds it, hence so little of the
 // height) and 0.5 us + 8.6 ns h beside them; a wave of pairs 0.235 and 3.6 us.  A kernel without work takes
 // 2.4 us, one of pairs 5; adding up the parts of a tile 3 us, 50 ns a row and 10 ns a row of its height.
-// Measured at both sides of the borders (rows x n x kdim): 128 x 4,096 x 4,096, one 64 high 10.9 us, two
-// parts 12.7; 16 x 4,096 x 4,096, four parts 7.7, one 10.0; 1,024 x 4,096 x 4,096, pairs 16.8, one 128 high
-// 21; 8,000 x 8,000 x 1,000, pairs 83, one 128 high 104; 4,096 x 1,024 x 1,024, both 9.3;
-// 4,096 x 65,536 x 128 to 32 bits, one 128 high 200, pairs 236.
+// Measured at both sides of the borders (rows x n x kdim, 16-bit results, calls in a row): 16 x 4,096 x 4,096, four parts
+// 6.9 us, one 9.1; 128 x 4,096 x 4,096, one 32 high 9.7, two parts 12.0; 777 x 1,000 x 960, one 64 high 5.1, 128 high 5.7;
+// 512 x 4,096 x 4,096, one 128 high 11.5, pairs 14.8; 1,024 x 4,096 x 4,096, pairs 15.5, one 128 high 19.5;
+// 4,096 x 1,024 x 1,024, 8.3 and 8.5; 8,000 x 8,000 x 1,000, pairs 68, one 128 high 104; 4,096 x 65,536 x 128 to 32 bits,
+// one 128 high 162, pairs 204.  The fit is older than the present epilogue: of 26 sizes it takes the fastest form or one
+// within 5 % in 25, and loses 10 % at 4,000 rows over 64 experts, 1,000 x 512 (13.7; one 128 high 12.4).
 template <typename T>
 cudaError_t Launch(const Operands& o, const MatmulArgs& a) {
     if (a.kdim == 0) {
